@@ -3,6 +3,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -30,17 +32,28 @@ def build(force=False, verbose=False):
     if not force and not needs_build():
         return LIB
     os.makedirs(LIBDIR, exist_ok=True)
-    cmd = [_hipcc(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
-           "-Wno-unused-value",
-           # no SLP vectorisation => no packed-f32 VALU (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32) in any kernel.  Found with several
-           # engines in flight (tools/inflight_lin.py): the LOW half of v_pk_fma_f32 results in the wide-K head kernel came out wrong
-           # (1e-3 .. 7e-2, a few elements, even rows = low halves only) whenever its waves shared a CU with another kernel's MFMA
-           # waves -- never alone, never with the scalar form.  The same IEEE results either way; packed f32 beside MFMAs is slower
-           # anyway (cdna_hip_programming.md, co-issue table).
-           "-fno-slp-vectorize"] + os.environ.get("W2C_EXTRA_HIPCC_FLAGS", "").split() + [os.path.join(CSRC, s) for s in SOURCES] + ["-o", LIB + ".tmp"]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
+    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
+             "-Wno-unused-value",
+             # no SLP vectorisation => no packed-f32 VALU (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32) in any kernel.  Found with several
+             # engines in flight (tools/inflight_lin.py): the LOW half of v_pk_fma_f32 results in the wide-K head kernel came out wrong
+             # (1e-3 .. 7e-2, a few elements, even rows = low halves only) whenever its waves shared a CU with another kernel's MFMA
+             # waves -- never alone, never with the scalar form.  The same IEEE results either way; packed f32 beside MFMAs is slower
+             # anyway (cdna_hip_programming.md, co-issue table).
+             "-fno-slp-vectorize",
+             # ... and none from explicit float2 / float4 arithmetic either: the target feature is off for every kernel
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + os.environ.get("W2C_EXTRA_HIPCC_FLAGS", "").split()
+    tmp = tempfile.mkdtemp(prefix="w2c_build_")
+    try:
+        objs = [os.path.join(tmp, os.path.splitext(s)[0] + ".o") for s in SOURCES]
+        cmds = [[_hipcc()] + flags + ["-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objs)]
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds), file=sys.stderr)
+        with ThreadPoolExecutor(max_workers=min(len(cmds), 8)) as pool:          # one hipcc per source file
+            for r in [pool.submit(subprocess.run, c, check=True) for c in cmds]:
+                r.result()
+        subprocess.run([_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC"] + objs + ["-o", LIB + ".tmp"], check=True)
+    finally:
+        shutil.rmtree(tmp, ignore_errors=True)
     check_no_packed_f32(LIB + ".tmp")
     os.replace(LIB + ".tmp", LIB)
     return LIB
@@ -58,7 +71,6 @@ PACKED_F32_FREE = ("linear_widek_kernel", "linear_kernel", "head_tail", "head_fc
 
 def check_no_packed_f32(lib, kernels=PACKED_F32_FREE):
     import re
-    import tempfile
     objdump = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_hipcc()))), "lib", "llvm", "bin", "llvm-objdump")
     if not os.path.exists(objdump):
         objdump = "/opt/rocm/lib/llvm/bin/llvm-objdump"
