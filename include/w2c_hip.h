@@ -504,6 +504,37 @@ int w2c_nchw_f32_to_nhwc_bf16(const float* x, int M, int C, int H, int W, uint16
 int w2c_nhwc_bf16_to_nchw_f32(const uint16_t* x, int x_cstride, int M, int C, int H, int W, float* y,
                               w2c_stream_t stream);
 
+/* ---- A model's head and its training step -------------------------------------------------------------------------------------
+ * Element types: dtype 0 = f32, 1 = bf16, 2 = f16.  Pointers need the alignment of one element. */
+
+/* Layer norm over the last dimension of [rows, cols], with an optional residual add in front of it:
+ *   h = x + residual (rounded to dtype; residual NULL: h = x and `h` is not written), y = (h - mean) * rstd * weight + bias.
+ * weight / bias: [cols] of wtype (0 = f32, or dtype) or NULL (1 / 0); mean, rstd: f32 [rows], for the backward.
+ * backward: dx = gradient of x and of residual (dh: gradient that reaches h by another way, added; or NULL), dweight / dbias [cols] of wtype
+ * (NULL: not wanted), workspace: w2c_layer_norm_workspace_bytes.  Deterministic (no atomics). */
+int w2c_layer_norm_forward(const void* x, const void* residual, int dtype, long long rows, int cols, const void* weight, const void* bias, int wtype,
+                           float eps, void* y, void* h, float* mean, float* rstd, w2c_stream_t stream);
+long long w2c_layer_norm_workspace_bytes(long long rows, int cols, int dtype);
+int w2c_layer_norm_backward(const void* dy, const void* h, const void* dh, int dtype, long long rows, int cols, const void* weight, int wtype,
+                            const float* mean, const float* rstd, void* dx, void* dweight, void* dbias, void* workspace, long long workspace_bytes,
+                            w2c_stream_t stream);
+
+/* Log probability of a given class, entropy and the `top` largest alternatives of every row of logits, one read of them.
+ * x: [outer, classes, inner]; inner = 1: rows of `row_stride` >= classes elements; inner > 1: dense (row_stride = classes * inner).  Rows are
+ * numbered outer * inner.  target: int64 [rows] or NULL (then logp NULL); ignore_index there answers 0, any other value outside
+ * [0, classes) NaN.  logp, entropy: f32 [rows]; top_logp f32, top_index int64 [rows, top], largest first, equal logits by the lower index
+ * (top <= 32, <= classes; a NaN counts as -inf in this order); stats: f32 [rows, 2], for the backward.  -inf is a masked class; a row of nothing else
+ * answers logp = -inf, entropy = 0 and has no gradient; NaN or +inf make a row's logp, entropy and top_logp NaN.
+ * backward: dx (dense) of g_logp [rows], g_entropy [rows], g_top [rows, top], each NULL where nothing flows back.  A top_index outside
+ * [0, classes) is skipped. */
+long long w2c_log_probs_workspace_bytes(long long outer, int classes, long long inner, int top);
+int w2c_log_probs_forward(const void* x, int dtype, long long outer, int classes, long long inner, long long row_stride, const long long* target,
+                          long long ignore_index, int top, float* logp, float* entropy, float* top_logp, long long* top_index, float* stats,
+                          void* workspace, long long workspace_bytes, w2c_stream_t stream);
+int w2c_log_probs_backward(const void* x, int dtype, long long outer, int classes, long long inner, long long row_stride, const long long* target,
+                           long long ignore_index, const float* stats, const float* entropy, int top, const long long* top_index,
+                           const float* g_logp, const float* g_entropy, const float* g_top, void* dx, w2c_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

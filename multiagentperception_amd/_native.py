@@ -90,6 +90,12 @@ SIGNATURES = {
     "w2c_confusion_matrix": [_vp, _i, _vp, _ll, _i, _vp, _vp],
     "w2c_nchw_f32_to_nhwc_bf16": [_vp, _i, _i, _i, _i, _vp, _i, _vp],
     "w2c_nhwc_bf16_to_nchw_f32": [_vp, _i, _i, _i, _i, _i, _vp, _vp],
+    "w2c_layer_norm_forward": [_vp, _vp, _i, _ll, _i, _vp, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp],
+    "w2c_layer_norm_workspace_bytes": [_ll, _i, _i],
+    "w2c_layer_norm_backward": [_vp, _vp, _vp, _i, _ll, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "w2c_log_probs_workspace_bytes": [_ll, _i, _ll, _i],
+    "w2c_log_probs_forward": [_vp, _i, _ll, _i, _ll, _ll, _vp, _ll, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "w2c_log_probs_backward": [_vp, _i, _ll, _i, _ll, _ll, _vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp],
 }
 
 _lib = None
@@ -120,8 +126,7 @@ def lib():
                 raise W2CError("libw2c_hip.so does not export %s (stale build?)" % name)
             fn.argtypes = argtypes
             fn.restype = (_c.c_char_p if name in ("w2c_status_string", "w2c_last_error_string") else
-                          _c.c_longlong if name in ("w2c_conv_splitk_workspace_bytes", "w2c_conv_wgrad_workspace_bytes", "w2c_bn_workspace_bytes",
-                                                     "w2c_cross_entropy2d_workspace_bytes", "w2c_stem_wgrad_workspace_bytes") else _i)
+                          _c.c_longlong if name.endswith("_workspace_bytes") else _i)
         _lib = handle
     return _lib
 

@@ -1,0 +1,88 @@
+// Shared by the kernels of a model's head and training step (layer_norm.hip, log_probs.hip, fp8_matmul.hip, adamw.hip): element types,
+// 16-byte accesses at any element alignment, wave reductions, power-of-two block scales.
+#pragma once
+#include "w2c_common.h"
+
+// element types of the C ABI
+enum { W2C_F32 = 0, W2C_BF16 = 1, W2C_F16 = 2 };
+
+namespace {
+
+struct bf16_t { uint16_t b; };
+struct f16_t { _Float16 h; };
+template <typename T> struct ElemOf;
+template <> struct ElemOf<float> { static constexpr int VEC = 4; };
+template <> struct ElemOf<bf16_t> { static constexpr int VEC = 8; };
+template <> struct ElemOf<f16_t> { static constexpr int VEC = 8; };
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16_t x) { return bf16_to_f32(x.b); }
+__device__ __forceinline__ float to_f32(f16_t x) { return (float)x.h; }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float x) { return bf16_t{f32_to_bf16(x)}; }
+template <> __device__ __forceinline__ f16_t from_f32<f16_t>(float x) { return f16_t{(_Float16)x}; }
+
+// N consecutive elements with the alignment of ONE element: rows of odd length and views into a row start anywhere, and this part's
+// global accesses of 16 bytes need no more than that.  (Split over two cache lines such an access costs one more request, no more.)
+template <typename T, int N> struct __attribute__((packed)) Pack { T v[N]; };
+template <typename T, int N> using PackAt = Pack<T, N> __attribute__((aligned(sizeof(T))));
+
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T* __restrict__ p, float (&v)[N]) {
+    PackAt<T, N> t;
+    __builtin_memcpy(&t, p, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32(t.v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T* __restrict__ p, const float (&v)[N]) {
+    PackAt<T, N> t;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t.v[i] = from_f32<T>(v[i]);
+    __builtin_memcpy(p, &t, sizeof(t));
+}
+// the same, of which only the first `n` elements exist (n <= 0: none; absent ones read as `fill`)
+template <typename T, int N>
+__device__ __forceinline__ void load_part(const T* __restrict__ p, long long n, float (&v)[N], float fill = 0.f) {
+    if (n >= N) load_n<T, N>(p, v);
+    else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < n ? to_f32(p[i]) : fill;
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_part(T* __restrict__ p, long long n, const float (&v)[N]) {
+    if (n >= N) store_n<T, N>(p, v);
+    else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n) p[i] = from_f32<T>(v[i]);
+    }
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// Block scales are powers of two, held as a biased exponent byte (e8m0: value 2^(b - 127), 255 = NaN): the matrix instructions take them as
+// they are, and scaling by one is exact.  The scale of a block is the smallest 2^e with amax <= TOP * 2^e, by the fields of the two
+// floats; a block of zeros has 2^0.  amax has to be finite and >= 0.
+constexpr float FP8_TOP = 448.f;                    // largest e4m3 value, 1.75 * 2^8
+__device__ __forceinline__ int scale_exponent(float amax) {
+    const uint32_t b = __float_as_uint(amax), t = __float_as_uint(FP8_TOP);
+    const int e = (int)(b >> 23) - (int)(t >> 23) + ((b & 0x7FFFFFu) > (t & 0x7FFFFFu) ? 1 : 0);
+    return amax > 0.f ? (e < -127 ? -127 : e) : 0;
+}
+__device__ __forceinline__ float pow2f(int e) {      // 2^e for -149 <= e <= 127 (e = -127 and below are subnormal)
+    return e >= -126 ? __uint_as_float((uint32_t)(e + 127) << 23) : __uint_as_float(1u << (e + 149));
+}
+
+}  // namespace

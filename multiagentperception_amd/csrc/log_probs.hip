@@ -1,0 +1,562 @@
+// Log probabilities of given classes, with the entropy and the top alternatives of every row, and the gradient to the logits.
+//
+//   m = max_j x_j,  s = sum_j exp(x_j - m),  u = sum_j exp(x_j - m) (x_j - m)          one walk: (m, s, u) is rescaled when m grows
+//   log p_j = (x_j - m) - log s,   H = log s - u / s,   alternatives: the largest x_j, equal ones by the lower index
+//   dx_j = a_t [j = t] + sum_i b_i [j = top_i] - p_j (a_t + sum_i b_i + c (log p_j + H))       a, b, c: gradients of log p_t, log p_top, H
+//
+// (m, log s) are kept apart for the backward: their sum would cost the last digits of p where the logits are large.  A masked class is -inf
+// (p = 0, no gradient); a row without any other class answers -inf, H = 0 and no gradient.  NaN or +inf make the row's answers NaN.  A target
+// outside [0, C) that is not ignore_index answers NaN.
+//
+// HBM-bound: one read forward, one read and one write backward.  Three shapes of work:
+//   lane per row   class dimension strided (label maps) or at most 64 classes: 64 neighbouring rows per wave, alternatives in registers
+//   wave per row   up to 2 048 contiguous classes
+//   block per row or per part of a row   longer; few long rows are split over blocks and joined by a second launch
+// Alternatives of the last two: every thread keeps the largest (value, index) of what it read; the k-th largest of those is a bound that
+// at most k threads reach, and only they look through their values again.
+#include "lm_common.h"
+
+namespace {
+
+constexpr float LP_L2E = 1.44269504088896340736f;
+constexpr float LP_FLOOR = -200.f;            // exp(-200) is 0 in f32: stands for -inf where 0 * -inf would be NaN
+constexpr int LP_TOP_MOST = 32, LP_SPLIT_MOST = 64;
+constexpr int LP_LANE_MOST = 64, LP_WAVE_MOST = 2048;      // classes
+
+__device__ __forceinline__ float exp_d(float d) { return __builtin_amdgcn_exp2f(d * LP_L2E); }
+
+struct Run {                                  // of the values seen so far
+    float m, s, u;
+};
+// max first, then the sums against it; m = -inf (nothing but masked values) counts from 0
+__device__ __forceinline__ void run_raise(Run& r, float m) {
+    if (m > r.m) {
+        const float d = r.m - m, f = exp_d(d);
+        r.u = f * (r.u + r.s * __builtin_fmaxf(d, LP_FLOOR));
+        r.s *= f;
+        r.m = m;
+    }
+}
+template <int N>
+__device__ __forceinline__ float max_of(const float (&x)[N]) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = __builtin_fmaxf(m, x[i]);
+    return m;
+}
+template <int N>
+__device__ __forceinline__ void run_add(Run& r, const float (&x)[N], float chunk_max) {
+    run_raise(r, chunk_max);
+    const float base = r.m == -INFINITY ? 0.f : r.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float d = x[i] - base, e = exp_d(d);
+        r.s += e;
+        r.u = fmaf(e, __builtin_fmaxf(d, LP_FLOOR), r.u);
+    }
+}
+__device__ __forceinline__ void run_to(Run& r, float m) {           // restate against a larger (or equal) maximum
+    run_raise(r, m);
+}
+__device__ __forceinline__ Run wave_join(Run r) {
+    run_to(r, wave_max(r.m));
+    r.s = wave_sum(r.s);
+    r.u = wave_sum(r.u);
+    return r;
+}
+
+// order of the alternatives: larger value first, then lower index; NaN ranks as -inf.  0 = none
+typedef unsigned long long key_t;
+__device__ __forceinline__ key_t key_of(float v, int index) {
+    const uint32_t b = __float_as_uint(v == v ? v : -INFINITY);
+    const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+    return ((key_t)(v == 0.f ? 0x80000000u : o) << 32) | (uint32_t)~index;          // -0 and +0 are one value
+}
+__device__ __forceinline__ int key_index(key_t k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ float key_value(key_t k) {
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ key_t wave_max_key(key_t k) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const key_t p = __shfl_xor(k, o, 64);
+        k = p > k ? p : k;
+    }
+    return k;
+}
+
+struct Out {                                  // where a row's answers go
+    const long long* target;
+    long long ignore;
+    int top;
+    float *logp, *entropy, *top_logp;
+    long long* top_index;
+    float* stats;
+};
+struct Stat {
+    float m, logs;
+};
+__device__ __forceinline__ Stat row_answer(const Run& r, const Out& o, long long row, int C, float xt) {
+    const bool empty = r.m == -INFINITY && r.s == 0.f;
+    const float m = r.m == -INFINITY ? 0.f : r.m, logs = empty ? INFINITY : logf(r.s);
+    o.stats[2 * row] = m;
+    o.stats[2 * row + 1] = logs;
+    o.entropy[row] = empty ? 0.f : logs - r.u / r.s;
+    if (o.logp) {
+        const long long t = o.target[row];
+        o.logp[row] = t == o.ignore ? 0.f : t < 0 || t >= C ? __builtin_nanf("") : (xt - m) - logs;
+    }
+    return Stat{m, logs};
+}
+
+// ---- lane per row ------------------------------------------------------------------------------------------------------------------------
+// row i of block row n: classes at x[n * outer_stride + i * row_stride + j * class_stride]
+template <typename T, int KMAX>
+__global__ __launch_bounds__(256) void lp_lane_forward_kernel(const T* __restrict__ x, long long P, long long outer, int C, long long outer_stride,
+                                                              long long row_stride, long long class_stride, Out o) {
+    constexpr int N = 8;
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= P) return;
+    for (long long n = blockIdx.y; n < outer; n += gridDim.y) {
+        const long long row = n * P + i;
+        const T* p = x + n * outer_stride + i * row_stride;
+        const long long t = o.logp ? o.target[row] : -1;
+        const float xt = t >= 0 && t < C ? to_f32(p[t * class_stride]) : 0.f;
+        Run r{-INFINITY, 0.f, 0.f};
+        float tv[KMAX > 0 ? KMAX : 1];
+        int ti[KMAX > 0 ? KMAX : 1];
+#pragma unroll
+        for (int k = 0; k < KMAX; ++k) {
+            tv[k] = -INFINITY;
+            ti[k] = -1;
+        }
+        for (int j = 0; j < C; j += N) {
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = j + e < C ? to_f32(p[(long long)(j + e) * class_stride]) : -INFINITY;
+            run_add<N>(r, v, max_of<N>(v));
+            if constexpr (KMAX > 0) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    float cv = v[e] == v[e] ? v[e] : -INFINITY;
+                    int ci = j + e;
+                    if (ci < C && (cv > tv[KMAX - 1] || ti[KMAX - 1] < 0)) {
+                        bool in = false;                       // once in its place everything behind moves down, equal values too
+#pragma unroll
+                        for (int k = 0; k < KMAX; ++k) {
+                            in = in || cv > tv[k] || ti[k] < 0;
+                            const float sv = tv[k];
+                            const int si = ti[k];
+                            tv[k] = in ? cv : sv;
+                            ti[k] = in ? ci : si;
+                            cv = in ? sv : cv;
+                            ci = in ? si : ci;
+                        }
+                    }
+                }
+            }
+        }
+        const Stat s = row_answer(r, o, row, C, xt);
+        if constexpr (KMAX > 0) {
+#pragma unroll
+            for (int k = 0; k < KMAX; ++k)
+                if (k < o.top) {
+                    o.top_logp[row * o.top + k] = (tv[k] - s.m) - s.logs;
+                    o.top_index[row * o.top + k] = ti[k];
+                }
+        }
+    }
+}
+
+// ---- wave or block per (part of a) row -----------------------------------------------------------------------------------------------------
+// The top keys of NW waves' rows' parts, by rounds of the largest: `mine` is a lane's key; afterwards lane l < k of the FIRST wave holds the
+// l-th largest of the block's elements >= the bound.  lists: k * k keys, firsts: NW * k keys, both in shared memory.
+template <typename T, int NW>
+__device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int hi, int t, key_t mine, int k, key_t* lists, key_t* firsts, int* count) {
+    constexpr int VEC = ElemOf<T>::VEC, TPR = NW * 64;
+    const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6;
+    key_t left = mine, bound = 0;
+    for (int r = 0; r < k; ++r) {                        // this wave's k largest thread keys
+        bound = wave_max_key(left);
+        if (left == bound) left = 0;                     // keys differ (the index is in them), 0 aside
+        if constexpr (NW > 1)
+            if (lane == 0) firsts[wave * k + r] = bound;
+    }
+    if constexpr (NW > 1) {
+        if (threadIdx.x == 0) *count = 0;
+        __syncthreads();
+        if (wave == 0) {                                 // the k-th largest of all waves' firsts
+            int at = 0;                                  // lane w < NW walks wave w's sorted list
+            for (int r = 0; r < k; ++r) {
+                const key_t head = lane < NW && at < k ? firsts[lane * k + at] : 0;
+                bound = wave_max_key(head);
+                if (head == bound) ++at;
+            }
+            if (lane == 0) firsts[0] = bound;            // (read by this wave only, above, before this write)
+        }
+        __syncthreads();
+        bound = firsts[0];
+    } else {
+        if (lane == 0) *count = 0;
+        __builtin_amdgcn_wave_barrier();
+    }
+    if (mine && mine >= bound) {                         // at most k threads
+        key_t* list = lists + (long long)atomicAdd(count, 1) * k;
+        int n = 0;
+        for (int c = lo + t * VEC; c < hi; c += TPR * VEC) {
+            float v[VEC];
+            load_part<T, VEC>(p + c, hi - c, v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const key_t q = c + e < hi ? key_of(v[e], c + e) : 0;
+                if (q >= bound && q && (n < k || q > list[n - 1])) {
+                    int at = n < k ? n++ : n - 1;
+                    for (; at > 0 && list[at - 1] < q; --at) list[at] = list[at - 1];
+                    list[at] = q;
+                }
+            }
+        }
+        for (; n < k; ++n) list[n] = 0;
+    }
+    if constexpr (NW > 1) __syncthreads();
+    else {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    }
+    key_t answer = 0;
+    if (wave == 0) {
+        const int lists_n = *count;
+        int at = 0;
+        for (int r = 0; r < k; ++r) {
+            const key_t head = lane < lists_n && at < k ? lists[lane * k + at] : 0;
+            const key_t best = wave_max_key(head);
+            if (head == best && head) ++at;
+            if (lane == r) answer = best;
+        }
+    }
+    return answer;
+}
+
+// parts == nullptr: the whole row is here.  Otherwise part blockIdx.y of it, and its (m, s, u) and k keys go to parts / part_keys
+// [row][part] for lp_join_kernel.
+template <typename T, int NW>
+__global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int part_len,
+                                                             Out o, float* __restrict__ parts, key_t* __restrict__ part_keys) {
+    constexpr int VEC = ElemOf<T>::VEC, TPR = NW * 64, ROWS = 256 / TPR;
+    extern __shared__ key_t shared[];                    // per row: k * k lists | (NW > 1: NW * k firsts) | count
+    __shared__ float slots[3][NW];
+    const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6, k = o.top;
+    const long long row = (long long)blockIdx.x * ROWS + (NW == 1 ? wave : 0);
+    if (row >= rows) return;                             // whole waves, and only where no barrier follows
+    const T* p = x + row * row_stride;
+    const int lo = blockIdx.y * part_len, hi = C - lo < part_len ? C : lo + part_len;
+    Run r{-INFINITY, 0.f, 0.f};
+    float best = -INFINITY;
+    int at = lo + t * VEC;
+    for (int c = lo + t * VEC; c < hi; c += TPR * VEC) {
+        float v[VEC];
+        load_part<T, VEC>(p + c, hi - c, v, -INFINITY);
+        const float cm = max_of<VEC>(v);
+        if (k && cm > best) {
+            best = cm;
+#pragma unroll
+            for (int e = VEC - 1; e >= 0; --e)
+                if (v[e] == cm) at = c + e;
+        }
+        run_add<VEC>(r, v, cm);
+    }
+    r = wave_join(r);
+    if constexpr (NW > 1) {
+        if ((threadIdx.x & 63) == 0) {
+            slots[0][wave] = r.m;
+            slots[1][wave] = r.s;
+            slots[2][wave] = r.u;
+        }
+        __syncthreads();
+        Run a{slots[0][0], slots[1][0], slots[2][0]};
+#pragma unroll
+        for (int i = 1; i < NW; ++i) {
+            Run b{slots[0][i], slots[1][i], slots[2][i]};
+            run_to(a, b.m);
+            run_to(b, a.m);
+            a.s += b.s;
+            a.u += b.u;
+        }
+        r = a;
+    }
+    Stat s{0.f, 0.f};
+    if (t == 0) {
+        if (parts) {
+            float* q = parts + (row * gridDim.y + blockIdx.y) * 3;
+            q[0] = r.m;
+            q[1] = r.s;
+            q[2] = r.u;
+        } else {
+            const long long g = o.logp ? o.target[row] : -1;
+            s = row_answer(r, o, row, C, g >= 0 && g < C ? to_f32(p[g]) : 0.f);
+        }
+    }
+    if (!k) return;
+    key_t* mem = shared + (NW == 1 ? wave * (k * k + 1) : 0);
+    const key_t mine = lo + t * VEC < hi ? key_of(best, at) : 0;
+    const key_t q = top_keys<T, NW>(p, lo, hi, t, mine, k, mem, mem + k * k, (int*)(mem + k * k + (NW == 1 ? 0 : NW * k)));
+    if (wave == 0 || NW == 1) {
+        s.m = __shfl(s.m, 0, 64);
+        s.logs = __shfl(s.logs, 0, 64);
+        if (t < k) {
+            if (parts) part_keys[(row * gridDim.y + blockIdx.y) * k + t] = q;
+            else {
+                o.top_logp[row * k + t] = (key_value(q) - s.m) - s.logs;
+                o.top_index[row * k + t] = key_index(q);
+            }
+        }
+    }
+}
+
+// one wave per row: lane l joins part l
+template <typename T>
+__global__ __launch_bounds__(256) void lp_join_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int n_parts, Out o,
+                                                      const float* __restrict__ parts, const key_t* __restrict__ part_keys) {
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, k = o.top;
+    if (row >= rows) return;
+    Run r{-INFINITY, 0.f, 0.f};
+    if (lane < n_parts) {
+        const float* q = parts + (row * n_parts + lane) * 3;
+        r = Run{q[0], q[1], q[2]};
+    }
+    r = wave_join(r);
+    Stat s{0.f, 0.f};
+    if (lane == 0) {
+        const long long g = o.logp ? o.target[row] : -1;
+        s = row_answer(r, o, row, C, g >= 0 && g < C ? to_f32(x[row * row_stride + g]) : 0.f);
+    }
+    if (!k) return;
+    s.m = __shfl(s.m, 0, 64);
+    s.logs = __shfl(s.logs, 0, 64);
+    int at = 0;
+    key_t answer = 0;
+    for (int i = 0; i < k; ++i) {
+        const key_t head = lane < n_parts && at < k ? part_keys[(row * n_parts + lane) * k + at] : 0;
+        const key_t best = wave_max_key(head);
+        if (head == best && head) ++at;
+        if (lane == i) answer = best;
+    }
+    if (lane < k) {
+        o.top_logp[row * k + lane] = (key_value(answer) - s.m) - s.logs;
+        o.top_index[row * k + lane] = key_index(answer);
+    }
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------------------------
+struct Grad {
+    const long long* target;
+    long long ignore;
+    const float *stats, *entropy, *g_logp, *g_entropy, *g_top;
+    const long long* top_index;
+    int top;
+};
+struct RowGrad {
+    float m, logs, H, a, whole, c;
+    long long t;
+    bool empty;
+};
+__device__ __forceinline__ RowGrad row_grad(const Grad& g, long long row, int C) {
+    RowGrad r;
+    r.m = g.stats[2 * row];
+    r.logs = g.stats[2 * row + 1];
+    r.H = g.entropy[row];
+    r.empty = r.logs == INFINITY;
+    r.t = -1;
+    r.a = 0.f;
+    if (g.g_logp) {
+        const long long t = g.target[row];
+        if (t != g.ignore) {
+            r.t = t;
+            r.a = t < 0 || t >= C ? __builtin_nanf("") : g.g_logp[row];
+        }
+    }
+    r.whole = r.a;
+    if (g.g_top)
+        for (int i = 0; i < g.top; ++i) r.whole += g.g_top[row * g.top + i];
+    r.c = g.g_entropy ? g.g_entropy[row] : 0.f;
+    return r;
+}
+__device__ __forceinline__ float class_grad(const RowGrad& r, float x, int j) {
+    const float l = (x - r.m) - r.logs, p = exp_d(l);
+    float d = p == 0.f ? 0.f : -p * fmaf(r.c, l + r.H, r.whole);
+    if (j == r.t) d += r.a;
+    return r.empty ? 0.f : d;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void lp_lane_backward_kernel(const T* __restrict__ x, long long P, long long outer, int C, long long outer_stride,
+                                                               long long row_stride, long long class_stride, Grad g, T* __restrict__ dx,
+                                                               long long dx_outer_stride, long long dx_row_stride) {
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= P) return;
+    for (long long n = blockIdx.y; n < outer; n += gridDim.y) {
+        const long long row = n * P + i;
+        const T* p = x + n * outer_stride + i * row_stride;
+        T* d = dx + n * dx_outer_stride + i * dx_row_stride;
+        const RowGrad r = row_grad(g, row, C);
+#pragma unroll 4
+        for (int j = 0; j < C; ++j) {
+            d[j * class_stride] = from_f32<T>(class_grad(r, to_f32(p[j * class_stride]), j));
+        }
+        if (g.g_top && !r.empty)
+            for (int k = 0; k < g.top; ++k) {            // the alternatives' own terms: the same thread writes those places again
+                const long long j = g.top_index[row * g.top + k];
+                if (j >= 0 && j < C) d[j * class_stride] = from_f32<T>(class_grad(r, to_f32(p[j * class_stride]), (int)j) + g.g_top[row * g.top + k]);
+            }
+    }
+}
+
+// a block (NW = 4) or a wave (NW = 1) per part of a row; the alternatives' own terms are put right by the block that wrote them
+template <typename T, int NW>
+__global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int part_len,
+                                                              Grad g, T* __restrict__ dx) {
+    constexpr int VEC = ElemOf<T>::VEC, TPR = NW * 64, ROWS = 256 / TPR;
+    const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const long long row = (long long)blockIdx.x * ROWS + (NW == 1 ? threadIdx.x >> 6 : 0);
+    if (row >= rows) return;
+    const T* p = x + row * row_stride;
+    T* d = dx + row * C;
+    const int lo = blockIdx.y * part_len, hi = C - lo < part_len ? C : lo + part_len;
+    const RowGrad r = row_grad(g, row, C);
+    for (int c = lo + t * VEC; c < hi; c += TPR * VEC) {
+        float v[VEC];
+        load_part<T, VEC>(p + c, hi - c, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = class_grad(r, v[e], c + e);
+        store_part<T, VEC>(d + c, hi - c, v);
+    }
+    if (!g.g_top || r.empty) return;
+    if constexpr (NW > 1) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+    if (t < g.top) {
+        const long long j = g.top_index[row * g.top + t];
+        if (j >= lo && j < hi) d[j] = from_f32<T>(class_grad(r, to_f32(p[j]), (int)j) + g.g_top[row * g.top + t]);
+    }
+}
+
+// few long rows: enough parts for about four blocks on every CU, none under 256 lanes' accesses of 16 bytes
+int lp_parts(long long rows, int C) {
+    if (C <= LP_WAVE_MOST) return 1;
+    long long n = (1024 + rows - 1) / rows;
+    const long long most = (C + 2047) / 2048;
+    if (n > most) n = most;
+    return (int)(n > LP_SPLIT_MOST ? LP_SPLIT_MOST : n < 1 ? 1 : n);
+}
+int lp_part_len(int C, int n) {                // a multiple of 8 elements
+    const long long len = ((long long)C + n - 1) / n;
+    return (int)((len + 7) / 8 * 8);
+}
+bool lp_lane(int C, long long inner) { return inner > 1 || C <= LP_LANE_MOST; }
+
+struct LaneGrid {
+    long long P, outer, outer_stride, row_stride, class_stride;
+    dim3 grid, block;
+};
+LaneGrid lane_grid(long long outer, int C, long long inner, long long row_stride) {
+    LaneGrid g;
+    if (inner > 1) g = {inner, outer, (long long)C * inner, 1, inner};
+    else g = {outer, 1, 0, row_stride, 1};
+    const int threads = g.P <= 64 ? 64 : 256;
+    g.block = dim3(threads);
+    g.grid = dim3((unsigned)((g.P + threads - 1) / threads), (unsigned)(g.outer < 65535 ? g.outer : 65535));
+    return g;
+}
+
+template <typename T>
+int lp_forward(const void* x, long long outer, int C, long long inner, long long row_stride, const Out& o, void* ws, hipStream_t st) {
+    if (lp_lane(C, inner)) {
+        const LaneGrid g = lane_grid(outer, C, inner, row_stride);
+#define LP_LANE(K) hipLaunchKernelGGL((lp_lane_forward_kernel<T, K>), g.grid, g.block, 0, st, (const T*)x, g.P, g.outer, C, g.outer_stride, g.row_stride, g.class_stride, o)
+        if (o.top == 0) LP_LANE(0);
+        else if (o.top <= 2) LP_LANE(2);
+        else if (o.top <= 8) LP_LANE(8);
+        else LP_LANE(32);
+#undef LP_LANE
+        return w2c_launch_status();
+    }
+    const int k = o.top;
+    if (C <= LP_WAVE_MOST) {
+        hipLaunchKernelGGL((lp_row_forward_kernel<T, 1>), dim3((unsigned)((outer + 3) / 4)), dim3(256), (size_t)4 * (k * k + 1) * sizeof(key_t), st,
+                           (const T*)x, outer, C, row_stride, C, o, (float*)nullptr, (key_t*)nullptr);
+        return w2c_launch_status();
+    }
+    const int n = lp_parts(outer, C);
+    const int len = n > 1 ? lp_part_len(C, n) : C, used = (int)(((long long)C + len - 1) / len);
+    key_t* keys = n > 1 ? (key_t*)ws : nullptr;
+    float* parts = n > 1 ? (float*)(keys + (long long)outer * n * k) : nullptr;
+    hipLaunchKernelGGL((lp_row_forward_kernel<T, 4>), dim3((unsigned)outer, used), dim3(256), (size_t)(k * k + 4 * k + 1) * sizeof(key_t), st,
+                       (const T*)x, outer, C, row_stride, len, o, parts, keys);
+    if (n > 1)
+        hipLaunchKernelGGL((lp_join_kernel<T>), dim3((unsigned)((outer + 3) / 4)), dim3(256), 0, st, (const T*)x, outer, C, row_stride, used, o,
+                           (const float*)parts, (const key_t*)keys);
+    return w2c_launch_status();
+}
+
+template <typename T>
+int lp_backward(const void* x, long long outer, int C, long long inner, long long row_stride, const Grad& g, void* dx, hipStream_t st) {
+    if (lp_lane(C, inner)) {
+        const LaneGrid l = lane_grid(outer, C, inner, row_stride);
+        hipLaunchKernelGGL((lp_lane_backward_kernel<T>), l.grid, l.block, 0, st, (const T*)x, l.P, l.outer, C, l.outer_stride, l.row_stride,
+                           l.class_stride, g, (T*)dx, l.outer_stride, inner > 1 ? 1ll : (long long)C);
+        return w2c_launch_status();
+    }
+    if (C <= LP_WAVE_MOST) {
+        hipLaunchKernelGGL((lp_row_backward_kernel<T, 1>), dim3((unsigned)((outer + 3) / 4)), dim3(256), 0, st, (const T*)x, outer, C, row_stride, C, g,
+                           (T*)dx);
+        return w2c_launch_status();
+    }
+    const int len = 256 * ElemOf<T>::VEC * 8;              // eight accesses per lane
+    hipLaunchKernelGGL((lp_row_backward_kernel<T, 4>), dim3((unsigned)outer, (C - 1) / len + 1), dim3(256), 0, st, (const T*)x, outer, C, row_stride,
+                       len, g, (T*)dx);
+    return w2c_launch_status();
+}
+
+bool lp_shape_ok(int dtype, long long outer, int C, long long inner, long long row_stride) {
+    return dtype >= W2C_F32 && dtype <= W2C_F16 && outer >= 1 && outer <= 0x7FFFFFFF && C >= 1 && C <= (1 << 28) && inner >= 1 &&
+           inner <= 0x7FFFFFFF && (inner > 1 ? row_stride == (long long)C * inner : row_stride >= C);
+}
+
+}  // namespace
+
+extern "C" long long w2c_log_probs_workspace_bytes(long long outer, int classes, long long inner, int top) {
+    if (!lp_shape_ok(W2C_F32, outer, classes, inner, (long long)classes * inner) || top < 0 || top > LP_TOP_MOST) return W2C_E_ARG;
+    const int n = lp_lane(classes, inner) ? 1 : lp_parts(outer, classes);
+    return n > 1 ? outer * n * ((long long)top * 8 + 12) : 0;
+}
+
+extern "C" int w2c_log_probs_forward(const void* x, int dtype, long long outer, int classes, long long inner, long long row_stride,
+                                     const long long* target, long long ignore_index, int top, float* logp, float* entropy, float* top_logp,
+                                     long long* top_index, float* stats, void* workspace, long long workspace_bytes, void* stream) {
+    if (!x || !entropy || !stats || !lp_shape_ok(dtype, outer, classes, inner, row_stride)) return W2C_E_ARG;
+    if ((target == nullptr) != (logp == nullptr) || top < 0 || top > LP_TOP_MOST || top > classes || (top && (!top_logp || !top_index))) return W2C_E_ARG;
+    const long long need = w2c_log_probs_workspace_bytes(outer, classes, inner, top);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))) return W2C_E_ARG;
+    w2c_clear_error();
+    const Out o{target, ignore_index, top, logp, entropy, top_logp, top_index, stats};
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == W2C_F32) return lp_forward<float>(x, outer, classes, inner, row_stride, o, workspace, st);
+    if (dtype == W2C_BF16) return lp_forward<bf16_t>(x, outer, classes, inner, row_stride, o, workspace, st);
+    return lp_forward<f16_t>(x, outer, classes, inner, row_stride, o, workspace, st);
+}
+
+extern "C" int w2c_log_probs_backward(const void* x, int dtype, long long outer, int classes, long long inner, long long row_stride,
+                                      const long long* target, long long ignore_index, const float* stats, const float* entropy, int top,
+                                      const long long* top_index, const float* g_logp, const float* g_entropy, const float* g_top, void* dx,
+                                      void* stream) {
+    if (!x || !stats || !entropy || !dx || !lp_shape_ok(dtype, outer, classes, inner, row_stride)) return W2C_E_ARG;
+    if ((g_logp && !target) || top < 0 || top > LP_TOP_MOST || top > classes || (g_top && (!top || !top_index))) return W2C_E_ARG;
+    w2c_clear_error();
+    const Grad g{target, ignore_index, stats, entropy, g_logp, g_entropy, g_top, top_index, top};
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == W2C_F32) return lp_backward<float>(x, outer, classes, inner, row_stride, g, dx, st);
+    if (dtype == W2C_BF16) return lp_backward<bf16_t>(x, outer, classes, inner, row_stride, g, dx, st);
+    return lp_backward<f16_t>(x, outer, classes, inner, row_stride, g, dx, st);
+}

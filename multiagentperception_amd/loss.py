@@ -11,6 +11,7 @@ package does not target (there is no HIP library involved on that branch, hence 
 """
 import functools
 import logging
+import typing
 
 import torch
 import torch.nn.functional as F
@@ -160,6 +161,64 @@ def bootstrapped_cross_entropy2d(input, target, K, weight=None, size_average=Tru
         px = F.cross_entropy(input, target, weight=weight, reduction="none", ignore_index=IGNORE_INDEX).view(batch_size, -1)
     topk, _ = px.topk(K, dim=1)
     return (topk.sum(dim=1) / K).sum() / float(batch_size)
+
+
+class LogProbs(typing.NamedTuple):
+    """what log_probs answers: f32 [...], f32 [...], f32 [..., top], int64 [..., top]; None where not asked for"""
+    logp: typing.Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logp: typing.Optional[torch.Tensor]
+    top_index: typing.Optional[torch.Tensor]
+
+
+class _LogProbsFn(torch.autograd.Function):
+    """log probability of the target, entropy and top alternatives: one read of the logits forward (w2c_log_probs_forward), one read and
+    one write backward (w2c_log_probs_backward)."""
+
+    @staticmethod
+    def forward(ctx, logits, target, top, dim, ignore_index):
+        ctx.set_materialize_grads(False)
+        r = ops.log_probs_forward(logits, target, top, dim, ignore_index)
+        ctx.save_for_backward(logits, target, *(t for t in r if t is not None))
+        ctx.there = [t is not None for t in r]
+        ctx.dim, ctx.ignore_index = dim, ignore_index
+        if r.top_index is not None:
+            ctx.mark_non_differentiable(r.top_index)
+        return r.logp, r.entropy, r.top_logp, r.top_index
+
+    @staticmethod
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, target, *rest = ctx.saved_tensors
+        r = ops.LogProbs(*(rest.pop(0) if there else None for there in ctx.there))
+        f32 = lambda g: None if g is None else g.float().contiguous()            # noqa: E731
+        d = ops.log_probs_backward(logits, target, r, f32(g_logp), f32(g_entropy), f32(g_top), ctx.dim, ctx.ignore_index)
+        return d, None, None, None, None
+
+
+def log_probs(input, target=None, top=0, dim=-1, ignore_index=-100):
+    """Log probability of `target` under the softmax of `input` along `dim`, the entropy, and the `top` largest log probabilities with their
+    classes (largest first, equal logits by the lower class), all differentiable but the classes.  input: logits (f32, bf16, f16), target:
+    integers of the other dimensions, `ignore_index` there answers 0.  -inf is a masked class; a row of nothing else answers logp = -inf, entropy 0
+    and has no gradient.  A target outside [0, n_classes) that is not `ignore_index` answers NaN.  Pixels of label maps: dim=1."""
+    if target is not None:
+        target = target.long().contiguous()
+    if input.is_cuda:
+        rows = input.dim() == 2 and dim % 2 == 1 and input.stride(1) == 1 and input.stride(0) >= input.shape[1]
+        return LogProbs(*_LogProbsFn.apply(input if rows else input.contiguous(), target, int(top), int(dim), int(ignore_index)))
+    x = input.float().movedim(dim, -1)
+    empty = (x == -float("inf")).all(-1, keepdim=True)
+    lp = torch.log_softmax(x.masked_fill(empty, 0.0), -1).masked_fill(empty, -float("inf"))
+    p = lp.exp()
+    entropy = -(p * lp.masked_fill(p == 0, 0.0)).sum(-1)
+    logp = top_logp = top_index = None
+    if target is not None:
+        inside = (target >= 0) & (target < x.shape[-1])
+        logp = lp.gather(-1, target.masked_fill(~inside, 0).unsqueeze(-1)).squeeze(-1)
+        logp = logp.masked_fill(~inside, float("nan")).masked_fill(target == ignore_index, 0.0)
+    if top:
+        top_index = x.masked_fill(x.isnan(), -float("inf")).sort(dim=-1, descending=True, stable=True)[1][..., :top]
+        top_logp = lp.gather(-1, top_index)
+    return LogProbs(logp, entropy, top_logp, top_index)
 
 
 key2loss = {

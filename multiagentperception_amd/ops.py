@@ -6,6 +6,7 @@ the tensor's device (so the path is re-entrant under DataParallel replicas and
 capturable in a graph).  There is no fallback: CPU tensors raise.
 """
 import threading
+import typing
 
 import torch
 
@@ -1773,3 +1774,185 @@ def nhwc_bf16_to_nchw_f32(x, channels=None):
         check(_native.lib().w2c_nhwc_bf16_to_nchw_f32(_p(x), cs, M, C, H, W, _p(y), _stream(dev)),
               "w2c_nhwc_bf16_to_nchw_f32")
     return y
+
+
+# ---- a model's head and its training step -----------------------------------------------------------------------------------------------
+
+_ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # the C ABI's element types
+
+
+def _elem(t, what):
+    code = _ELEM.get(t.dtype)
+    if code is None:
+        raise W2CError("%s: f32, bf16 or f16 expected, got %s" % (what, t.dtype))
+    return code
+
+
+def _ln_affine(x, weight, bias, what):
+    """(cols, element type of weight / bias) of a layer norm over x's last dimension"""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise W2CError("%s: the last dimension must have at least one element, got %s" % (what, tuple(x.shape)))
+    cols, wtype = x.shape[-1], None
+    for t in (weight, bias):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != cols or (t.dtype != torch.float32 and t.dtype != x.dtype) or (wtype is not None and t.dtype != wtype):
+            raise W2CError("%s: weight and bias must be [%d], both f32 or both %s" % (what, cols, x.dtype))
+        wtype = t.dtype
+    return cols, (torch.float32 if wtype is None else wtype)
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """x [..., D] f32 / bf16 / f16 -> (y, h, mean f32 [...], rstd f32 [...]): y = (h - mean) * rstd * weight + bias over the last dimension,
+    h = x + residual rounded to x's type (without residual h IS x).  include/w2c_hip.h w2c_layer_norm_forward."""
+    dev = _need_gpu(x, weight, bias, residual)
+    code = _elem(x, "layer_norm")
+    cols, wtype = _ln_affine(x, weight, bias, "layer_norm")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise W2CError("layer_norm: residual must have x's shape and type")
+    rows = x.numel() // cols
+    y = _empty(x.shape, x.dtype, dev)
+    h = _empty(x.shape, x.dtype, dev) if residual is not None else x
+    mean, rstd = _empty(x.shape[:-1], torch.float32, dev), _empty(x.shape[:-1], torch.float32, dev)
+    if rows:
+        with torch.cuda.device(dev):
+            check(_native.lib().w2c_layer_norm_forward(_p(x), _p(residual), code, rows, cols, _p(weight), _p(bias), _ELEM[wtype], float(eps),
+                                                       _p(y), _p(h) if residual is not None else None, _p(mean), _p(rstd), _stream(dev)),
+                  "w2c_layer_norm_forward")
+    return y, h, mean, rstd
+
+
+def layer_norm_backward(dy, h, weight, mean, rstd, dh=None, bias=True):
+    """-> (dx, dweight | None, dbias | None) of layer_norm_forward; dx is the gradient of x and of residual alike.  dh: the gradient that
+    reaches h by another way (the residual stream), added to dx.  weight None: no dweight (dbias then is f32)."""
+    dev = _need_gpu(dy, h, weight, mean, rstd, dh)
+    code = _elem(h, "layer_norm backward")
+    cols, wtype = _ln_affine(h, weight, None, "layer_norm backward")
+    rows = h.numel() // cols
+    for t in (dy, dh):
+        if t is not None and (t.shape != h.shape or t.dtype != h.dtype):
+            raise W2CError("layer_norm backward: dy and dh must have h's shape and type")
+    if mean.numel() != rows or rstd.numel() != rows or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise W2CError("layer_norm backward: mean and rstd must be f32, one per row")
+    dx = torch.empty_like(h)
+    dw = torch.empty(cols, dtype=wtype, device=dev) if weight is not None else None
+    db = torch.empty(cols, dtype=wtype, device=dev) if bias else None
+    if not rows:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+        return dx, dw, db
+    lib = _native.lib()
+    ws, nbytes = None, 0
+    if dw is not None or db is not None:
+        nbytes = lib.w2c_layer_norm_workspace_bytes(rows, cols, code)
+        if nbytes < 0:
+            raise W2CError("layer_norm backward: %d rows of %d are out of range" % (rows, cols))
+        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        check(lib.w2c_layer_norm_backward(_p(dy), _p(h), _p(dh), code, rows, cols, _p(weight), _ELEM[wtype], _p(mean), _p(rstd), _p(dx), _p(dw),
+                                          _p(db), _p(ws), nbytes, _stream(dev)), "w2c_layer_norm_backward")
+    return dx, dw, db
+
+
+LOG_PROBS_TOP_MOST = 32
+_LOG_PROBS_INNER_MOST = 1024       # classes: a longer class dimension that is not the last one is laid out last first (one thread walks a row there)
+
+
+class LogProbs(typing.NamedTuple):
+    """what log_probs_forward answers; `stats` (f32 [..., 2]) is for log_probs_backward"""
+    logp: typing.Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logp: typing.Optional[torch.Tensor]
+    top_index: typing.Optional[torch.Tensor]
+    stats: torch.Tensor
+
+
+def _class_rows(x, dim, what):
+    """(outer, classes, inner, row stride, shape of the rows) of logits with the classes along `dim`"""
+    if not -x.dim() <= dim < x.dim():
+        raise W2CError("%s: dim %d of a %d-dimensional tensor" % (what, dim, x.dim()))
+    dim %= x.dim()
+    rest = tuple(x.shape[:dim]) + tuple(x.shape[dim + 1:])
+    outer, inner = 1, 1
+    for n in x.shape[:dim]:
+        outer *= n
+    for n in x.shape[dim + 1:]:
+        inner *= n
+    classes = x.shape[dim]
+    if classes < 1:
+        raise W2CError("%s: no classes along dim %d of %s" % (what, dim, tuple(x.shape)))
+    if x.is_contiguous():
+        stride = classes * inner
+    elif x.dim() == 2 and dim == 1 and x.stride(1) == 1 and x.stride(0) >= classes:      # rows of a wider tensor (a padded vocabulary)
+        stride = x.stride(0)
+    else:
+        raise W2CError("%s: logits must be contiguous, or rows with contiguous classes" % what)
+    return outer, classes, inner, stride, rest
+
+
+def _log_probs_target(target, rest, dev, what):
+    if target is not None and (target.dtype != torch.int64 or tuple(target.shape) != rest or target.device != dev or not target.is_contiguous()):
+        raise W2CError("%s: target must be a contiguous int64 tensor of shape %s on the logits' device" % (what, rest))
+
+
+def log_probs_forward(logits, target=None, top=0, dim=-1, ignore_index=-100):
+    """logits f32 / bf16 / f16 with the classes along `dim` (contiguous, or 2-D rows of a wider tensor), target int64 of the other dimensions
+    or None -> LogProbs: logp f32 (0 where target is ignore_index), entropy f32, the `top` largest log probabilities f32 [..., top] and their
+    classes int64, largest first, equal logits by the lower class.  include/w2c_hip.h w2c_log_probs_forward."""
+    if not logits.is_cuda:
+        _need_gpu(logits)
+    dev = logits.device
+    code = _elem(logits, "log_probs")
+    outer, classes, inner, stride, rest = _class_rows(logits, dim, "log_probs")
+    _log_probs_target(target, rest, dev, "log_probs")
+    if not 0 <= top <= min(classes, LOG_PROBS_TOP_MOST):
+        raise W2CError("log_probs: top must lie in 0 .. min(classes, %d), got %d of %d classes" % (LOG_PROBS_TOP_MOST, top, classes))
+    if inner > 1 and classes > _LOG_PROBS_INNER_MOST:
+        return log_probs_forward(logits.movedim(dim, -1).contiguous(), target, top, -1, ignore_index)
+    logp = _empty(rest, torch.float32, dev) if target is not None else None
+    entropy, stats = _empty(rest, torch.float32, dev), _empty(rest + (2,), torch.float32, dev)
+    top_logp = _empty(rest + (top,), torch.float32, dev) if top else None
+    top_index = _empty(rest + (top,), torch.int64, dev) if top else None
+    if outer * inner:
+        lib = _native.lib()
+        nbytes = lib.w2c_log_probs_workspace_bytes(outer, classes, inner, top)
+        if nbytes < 0:
+            raise W2CError("log_probs: %d x %d x %d logits are out of range" % (outer, classes, inner))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with torch.cuda.device(dev):
+            check(lib.w2c_log_probs_forward(_p(logits), code, outer, classes, inner, stride, _p(target), int(ignore_index), top, _p(logp), _p(entropy),
+                                            _p(top_logp), _p(top_index), _p(stats), _p(ws), nbytes, _stream(dev)), "w2c_log_probs_forward")
+    return LogProbs(logp, entropy, top_logp, top_index, stats)
+
+
+def log_probs_backward(logits, target, forward, g_logp=None, g_entropy=None, g_top=None, dim=-1, ignore_index=-100):
+    """-> d logits (contiguous, logits' type) of log_probs_forward's logp, entropy and top_logp (f32 gradients of their shapes, or None);
+    `forward`: the LogProbs that it answered for these logits."""
+    if not logits.is_cuda:
+        _need_gpu(logits)
+    dev = logits.device
+    code = _elem(logits, "log_probs backward")
+    outer, classes, inner, stride, rest = _class_rows(logits, dim, "log_probs backward")
+    _log_probs_target(target, rest, dev, "log_probs backward")
+    if g_logp is not None and target is None:
+        raise W2CError("log_probs backward: a gradient of logp needs the target")
+    if g_top is not None and forward.top_index is None:
+        raise W2CError("log_probs backward: a gradient of the alternatives needs a forward with them")
+    top = 0 if forward.top_index is None else forward.top_index.shape[-1]
+    for t, shape in ((g_logp, rest), (g_entropy, rest), (g_top, rest + (top,)), (forward.stats, rest + (2,)), (forward.entropy, rest)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous()):
+            raise W2CError("log_probs backward: contiguous f32 tensors of the forward's shapes on the logits' device expected")
+    if forward.top_index is not None and (tuple(forward.top_index.shape) != rest + (top,) or forward.top_index.dtype != torch.int64
+                                          or forward.top_index.device != dev or not forward.top_index.is_contiguous()):
+        raise W2CError("log_probs backward: top_index is not the forward's")
+    if inner > 1 and classes > _LOG_PROBS_INNER_MOST:
+        d = log_probs_backward(logits.movedim(dim, -1).contiguous(), target, forward, g_logp, g_entropy, g_top, -1, ignore_index)
+        return d.movedim(-1, dim).contiguous()
+    dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    if outer * inner:
+        with torch.cuda.device(dev):
+            check(_native.lib().w2c_log_probs_backward(_p(logits), code, outer, classes, inner, stride, _p(target), int(ignore_index),
+                                                       _p(forward.stats), _p(forward.entropy), top, _p(forward.top_index), _p(g_logp),
+                                                       _p(g_entropy), _p(g_top), _p(dx), _stream(dev)), "w2c_log_probs_backward")
+    return dx

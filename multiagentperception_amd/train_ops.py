@@ -334,6 +334,59 @@ def maxpool3x3s2(pool, x):
     return pool(x)
 
 
+class _LayerNormFn(torch.autograd.Function):
+    """layer norm over the last dimension with an optional residual add in front (w2c_layer_norm_forward / _backward) -> (y, h)"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, residual):
+        ctx.set_materialize_grads(False)
+        y, h, mean, rstd = ops.layer_norm_forward(x.contiguous(), None if weight is None else weight.detach().contiguous(),
+                                                  None if bias is None else bias.detach().contiguous(), eps,
+                                                  None if residual is None else residual.contiguous())
+        ctx.save_for_backward(h, weight, bias, mean, rstd)
+        ctx.has_res = residual is not None
+        return (y, h) if ctx.has_res else (y, None)
+
+    @staticmethod
+    def backward(ctx, dy, dh):
+        h, weight, bias, mean, rstd = ctx.saved_tensors
+        dw = db = None
+        if dy is None:                                   # only h was used
+            dx = dh
+        else:
+            want_b = bias is not None and ctx.needs_input_grad[2]
+            dx, dw, db = ops.layer_norm_backward(dy.contiguous(), h, None if weight is None else weight.detach().contiguous(), mean, rstd,
+                                                 dh=None if dh is None else dh.contiguous(), bias=want_b)
+            if want_b:
+                db = db.to(bias.dtype)
+        return dx, dw, db, None, dx if ctx.has_res else None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """y = layer norm of h = x (+ residual) over the last dimension; with a residual -> (y, h).  HIP kernels under the "hip" backend on GPU
+    tensors (f32, bf16, f16; weight / bias f32 or x's type), stock ops otherwise."""
+    if _backend == "hip" and x.is_cuda:
+        y, h = _LayerNormFn.apply(x, weight, bias, float(eps), residual)
+        return y if residual is None else (y, h)
+    h = x if residual is None else x + residual
+    cast = lambda t: None if t is None else t.to(h.dtype)                       # noqa: E731
+    y = F.layer_norm(h, h.shape[-1:], cast(weight), cast(bias), eps)
+    return y if residual is None else (y, h)
+
+
+class LayerNormHip(nn.LayerNorm):
+    """nn.LayerNorm over the last dimension (same parameters, same state_dict keys) on layer_norm(); forward(x, residual) -> (y, h)."""
+
+    def __init__(self, normalized_shape, **kw):
+        super().__init__(normalized_shape, **kw)
+        if len(self.normalized_shape) != 1:
+            raise ops.W2CError("LayerNormHip: normalises over the last dimension only, got %s" % (tuple(self.normalized_shape),))
+
+    def forward(self, x, residual=None):
+        if x.shape[-1] != self.normalized_shape[0]:
+            raise ops.W2CError("LayerNormHip: %d features expected, got %s" % (self.normalized_shape[0], tuple(x.shape)))
+        return layer_norm(x, self.weight, self.bias, self.eps, residual)
+
 
 class GraphedTrainStep:
     """One whole training step -- forward, loss, backward, optimizer step -- captured into ONE HIP graph and replayed (round 4
