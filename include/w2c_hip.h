@@ -535,6 +535,23 @@ int w2c_log_probs_backward(const void* x, int dtype, long long outer, int classe
                            long long ignore_index, const float* stats, const float* entropy, int top, const long long* top_index,
                            const float* g_logp, const float* g_entropy, const float* g_top, void* dx, w2c_stream_t stream);
 
+/* One AdamW step over n tensors.  tensors: HOST array of n rows of nine int64: {p, g, m, v, m_scale, v_scale, step, elements, dtype}, device
+ * addresses but the last two; p and g of dtype; step f32 [1], the number of steps done, advanced by the call.
+ *   state_bits 32: m, v f32 [elements] (first and second moment), the two scales unused
+ *   state_bits  8: m, v e4m3 codes of the first moment and of the ROOT of the second, m_scale / v_scale e8m0 [ceil(elements / 256)]; rounded up
+ *                  or down at random by a hash of (seed, step, place); codes of values that are not finite are NaN
+ * lr: lr_dev[0] (f32) where lr_dev is not NULL, so that a captured step follows it.  n_squares > 0: the gradients are scaled by
+ * min(1, max_norm / (norm + 1e-6)), norm = sqrt(sum of squares), written to `norm` (f32 [1]) unless NULL; squares come from
+ * w2c_grad_squares over all gradients that share the norm (same rows; only g, elements and dtype are read), w2c_grad_squares_count of them.
+ * No row may share p, m, v or step with another.  workspace: w2c_adamw_workspace_bytes(n), 16-byte aligned, not shared with a call that
+ * may run at the same time.  Deterministic. */
+int w2c_grad_squares_count(const long long* tensors, int n);
+int w2c_grad_squares(const long long* tensors, int n, double* squares, int count, w2c_stream_t stream);
+long long w2c_adamw_workspace_bytes(int n);
+int w2c_adamw_step(const long long* tensors, int n, int state_bits, double lr, const float* lr_dev, double beta1, double beta2, double eps,
+                   double weight_decay, const double* squares, int n_squares, double max_norm, float* norm, unsigned seed, void* workspace,
+                   long long workspace_bytes, w2c_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -93,6 +93,11 @@ SIGNATURES = {
     "w2c_layer_norm_forward": [_vp, _vp, _i, _ll, _i, _vp, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp],
     "w2c_layer_norm_workspace_bytes": [_ll, _i, _i],
     "w2c_layer_norm_backward": [_vp, _vp, _vp, _i, _ll, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "w2c_grad_squares_count": [_vp, _i],
+    "w2c_grad_squares": [_vp, _i, _vp, _i, _vp],
+    "w2c_adamw_workspace_bytes": [_i],
+    "w2c_adamw_step": [_vp, _i, _i, _c.c_double, _vp, _c.c_double, _c.c_double, _c.c_double, _c.c_double, _vp, _i, _c.c_double, _vp, _c.c_uint,
+                       _vp, _ll, _vp],
     "w2c_log_probs_workspace_bytes": [_ll, _i, _ll, _i],
     "w2c_log_probs_forward": [_vp, _i, _ll, _i, _ll, _ll, _vp, _ll, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
     "w2c_log_probs_backward": [_vp, _i, _ll, _i, _ll, _ll, _vp, _ll, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp],

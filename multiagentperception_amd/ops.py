@@ -5,6 +5,7 @@ hands raw device pointers + sizes to libw2c_hip.so on torch's CURRENT stream of
 the tensor's device (so the path is re-entrant under DataParallel replicas and
 capturable in a graph).  There is no fallback: CPU tensors raise.
 """
+import ctypes
 import threading
 import typing
 
@@ -1956,3 +1957,117 @@ def log_probs_backward(logits, target, forward, g_logp=None, g_entropy=None, g_t
                                                        _p(forward.stats), _p(forward.entropy), top, _p(forward.top_index), _p(g_logp),
                                                        _p(g_entropy), _p(g_top), _p(dx), _stream(dev)), "w2c_log_probs_backward")
     return dx
+
+
+ADAMW_STATE_BLOCK = 256            # elements of a tensor that share a scale in an 8-bit moment
+
+
+def _dense(t):
+    """no gaps and no element twice: the elements in memory order are the tensor's elements"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda d: d[1]):
+        if s != want:
+            return False
+        want *= n
+    return True
+
+
+def _adamw_rows(params, grads, moments, steps):
+    """the C ABI's rows of nine int64 per tensor, after the checks that all four lists share"""
+    n = len(params)
+    if not n or len(grads) != n:
+        raise W2CError("adamw: as many gradients as parameters expected, at least one (got %d and %d)" % (len(grads), n))
+    dev = params[0].device
+    if dev.type != "cuda":
+        raise W2CError("w2c ops run only on an MI355X device tensor (got %s); there is no CPU fallback" % dev)
+    rows = []
+    for i, (p, g) in enumerate(zip(params, grads)):
+        code = _ELEM.get(p.dtype)
+        if code is None or g.dtype != p.dtype:
+            raise W2CError("adamw: parameter %d: f32, bf16 or f16 with a gradient of its type expected, got %s and %s" % (i, p.dtype, g.dtype))
+        if g.layout != torch.strided or g.shape != p.shape or g.device != dev or p.device != dev:
+            raise W2CError("adamw: parameter %d: a dense gradient of its shape on %s expected" % (i, dev))
+        if not (p.is_contiguous() and g.is_contiguous()) and (p.stride() != g.stride() or not _dense(p)):
+            raise W2CError("adamw: parameter %d and its gradient must be laid out alike, without gaps" % i)
+        m = moments[i] if moments is not None else (0, 0, 0, 0)
+        rows += (p.data_ptr(), g.data_ptr(), *m, steps[i] if steps is not None else 0, p.numel(), code)
+    return dev, (ctypes.c_longlong * len(rows))(*rows)
+
+
+def grad_squares(grads):
+    """sums of the squares of parts of the gradients (f64), for adamw_step's `squares`: their total is the squared norm of all of them"""
+    dev, rows = _adamw_rows(grads, grads, None, None)
+    count = _native.lib().w2c_grad_squares_count(rows, len(grads))
+    if count < 0:
+        raise W2CError("grad_squares: a tensor is too large")
+    out = torch.zeros(1, dtype=torch.float64, device=dev) if count == 0 else torch.empty(count, dtype=torch.float64, device=dev)
+    if count:
+        with torch.cuda.device(dev):
+            check(_native.lib().w2c_grad_squares(rows, len(grads), _p(out), count, _stream(dev)), "w2c_grad_squares")
+    return out
+
+
+def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, max_norm=None, seed=0, squares=None):
+    """One AdamW step in place over lists of tensors (include/w2c_hip.h w2c_adamw_step).
+    params f32 / bf16 / f16 with gradients of their types; steps: one f32 element each, advanced by the call; states, all alike:
+      (m, v)                    f32, laid out like the parameter
+      (m, m_scale, v, v_scale)  8 bits: m and the ROOT of v as float8_e4m3fn of the parameter's elements in memory order, float8_e8m0fnu
+                                scales of ADAMW_STATE_BLOCK elements; rounded at random by (seed, step, place)
+    lr: a number, or an f32 device tensor of one element (a captured step then follows it).  max_norm: the gradients are scaled down to this
+    norm in all; `squares` (grad_squares) where more tensors than these share the norm.  -> the norm before that (f32 on the device), or None."""
+    n = len(params)
+    if len(states) != n or len(steps) != n:
+        raise W2CError("adamw: %d parameters, %d states, %d steps" % (n, len(states), len(steps)))
+    bits = 32 if n and len(states[0]) == 2 else 8
+    moments = []
+    for i, (p, st) in enumerate(zip(params, states)):
+        if len(st) != (2 if bits == 32 else 4) or any(t.device != p.device for t in st):
+            raise W2CError("adamw: the states must all be (m, v) or all (m, m_scale, v, v_scale), on the parameters' device")
+        k = p.numel()
+        if bits == 32:
+            m, v = st
+            for t in st:
+                if t.dtype != torch.float32 or t.numel() != k or not (p.is_contiguous() and t.is_contiguous() or t.stride() == p.stride()):
+                    raise W2CError("adamw: parameter %d: f32 moments laid out like it expected" % i)
+            moments.append((m.data_ptr(), v.data_ptr(), 0, 0))
+        else:
+            m, ms, v, vs = st
+            blocks = -(-k // ADAMW_STATE_BLOCK)
+            if (m.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or ms.dtype != torch.float8_e8m0fnu or vs.dtype != torch.float8_e8m0fnu
+                    or m.numel() != k or v.numel() != k or ms.numel() != blocks or vs.numel() != blocks
+                    or not (m.is_contiguous() and v.is_contiguous() and ms.is_contiguous() and vs.is_contiguous())):
+                raise W2CError("adamw: parameter %d: contiguous float8_e4m3fn moments of %d and float8_e8m0fnu scales of %d expected" % (i, k, blocks))
+            moments.append((m.data_ptr(), v.data_ptr(), ms.data_ptr(), vs.data_ptr()))
+    for i, t in enumerate(steps):
+        if t.dtype != torch.float32 or t.numel() != 1 or t.device != params[i].device:
+            raise W2CError("adamw: parameter %d: its step must be one f32 element on its device" % i)
+    counters = [t.data_ptr() for t in steps]
+    dev, rows = _adamw_rows(params, grads, moments, counters)
+    written = [rows[9 * i] for i in range(n) if rows[9 * i + 7]]
+    if len(set(written)) != len(written) or len(set(counters)) != n or len({a for m in moments for a in m if a}) != sum(1 for m in moments for a in m if a):
+        raise W2CError("adamw: a parameter, moment or step is in the lists twice")
+    if max_norm is not None and not max_norm > 0:
+        raise W2CError("adamw: max_norm must be positive, got %r" % (max_norm,))
+    lr_dev = None
+    if torch.is_tensor(lr):
+        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
+            raise W2CError("adamw: a tensor lr must be one f32 element on the parameters' device")
+        lr_dev, lr = lr, 0.0
+    norm = None
+    if max_norm is not None:
+        if squares is None:
+            squares = grad_squares(grads)
+        elif squares.dtype != torch.float64 or squares.device != dev or not squares.is_contiguous() or not squares.numel():
+            raise W2CError("adamw: squares must come from grad_squares")
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+    lib = _native.lib()
+    nbytes = lib.w2c_adamw_workspace_bytes(n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        check(lib.w2c_adamw_step(rows, n, bits, float(lr), _p(lr_dev), float(beta1), float(beta2), float(eps), float(weight_decay),
+                                 _p(squares) if norm is not None else None, squares.numel() if norm is not None else 0, float(max_norm or 0.0),
+                                 _p(norm), int(seed) & 0xFFFFFFFF, _p(ws), nbytes, _stream(dev)), "w2c_adamw_step")
+    torch.autograd.graph.increment_version(params)           # the engines' packed weights and autograd notice the in-place write
+    return norm
