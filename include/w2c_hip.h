@@ -552,6 +552,20 @@ int w2c_adamw_step(const long long* tensors, int n, int state_bits, double lr, c
                    double weight_decay, const double* squares, int n_squares, double max_norm, float* norm, unsigned seed, void* workspace,
                    long long workspace_bytes, w2c_stream_t stream);
 
+/* 8-bit product with a power-of-two scale per 128 of the reduction: c[m][n] = sum_k a[m][k] 2^(sa - 127) b[n][k] 2^(sb - 127) (+ bias[n]), c [M, N] of
+ * dtype.  a [M, K], b [N, K]: e4m3fn codes, rows padded with zero codes to K, a multiple of 128, 16-byte aligned; a_scale e8m0
+ * [a_tile = 1: M | 128: ceil(M / 128)][K / 128], b_scale alike: a scale per row or per 128 rows.  f32 accumulation, deterministic. */
+int w2c_matmul_fp8(const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
+                   const float* bias, void* c, int dtype, w2c_stream_t stream);
+/* The codes and scales of x [rows, cols] (row stride `stride` elements): by rows (codes [rows, cols padded to 128], scale [rows, or ceil(rows / 128)
+ * with tile 128][ceil(cols / 128)]), of the transposed x (codes_t [cols, rows padded to 128], 16-byte aligned, scale_t alike), either NULL if not
+ * wanted, from one read.  A scale is the smallest power of two with amax <= 448 * scale, amax over the block's finite values (1 for zeros);
+ * codes round to nearest even; values that are not finite become NaN.  column_sums: f32 [cols] = sums of x over its rows, or NULL (with it:
+ * workspace of w2c_quantize_fp8_workspace_bytes). */
+long long w2c_quantize_fp8_workspace_bytes(long long rows, long long cols);
+int w2c_quantize_fp8(const void* x, int dtype, long long rows, long long cols, long long stride, int tile, void* codes, void* scale, void* codes_t,
+                     void* scale_t, float* column_sums, void* workspace, long long workspace_bytes, w2c_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

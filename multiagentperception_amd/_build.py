@@ -11,7 +11,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libw2c_hip.so")
 SOURCES = ["conv_igemm.hip", "conv_wgrad.hip", "bn_train.hip", "stem.hip", "stem_train.hip", "comm_attn.hip", "upsample.hip", "loss.hip", "layer_norm.hip",
-           "log_probs.hip", "adamw.hip"]
+           "log_probs.hip", "adamw.hip", "fp8_matmul.hip"]
 
 
 def _hipcc():

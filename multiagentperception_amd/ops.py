@@ -2071,3 +2071,86 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
                                  _p(norm), int(seed) & 0xFFFFFFFF, _p(ws), nbytes, _stream(dev)), "w2c_adamw_step")
     torch.autograd.graph.increment_version(params)           # the engines' packed weights and autograd notice the in-place write
     return norm
+
+
+FP8_BLOCK = 128                    # elements of the reduction that share a scale in matmul_fp8
+
+
+class Fp8Blocks(typing.NamedTuple):
+    """a matrix [rows, cols] in 8 bits: codes float8_e4m3fn [rows, cols padded with zeros to a multiple of 128], scale float8_e8m0fnu (powers
+    of two) [rows, or ceil(rows / 128) where 128 rows share them][padded cols / 128]"""
+    codes: torch.Tensor
+    scale: torch.Tensor
+    cols: int
+
+
+class Fp8Quantized(typing.NamedTuple):
+    rows: typing.Optional[Fp8Blocks]
+    columns: typing.Optional[Fp8Blocks]
+    sums: typing.Optional[torch.Tensor]
+
+
+def _fp8_new(rows, cols, tile, dev):
+    codes = _empty((rows, -(-cols // FP8_BLOCK) * FP8_BLOCK), torch.float8_e4m3fn, dev)
+    return Fp8Blocks(codes, _empty((-(-rows // tile), codes.shape[1] // FP8_BLOCK), torch.float8_e8m0fnu, dev), cols)
+
+
+def quantize_fp8(x, tile=1, rows=True, columns=False, sums=False):
+    """x f32 / bf16 / f16 [R, C] (its rows may be those of a wider tensor) -> Fp8Quantized: x by rows (to multiply along C), the transposed x (to
+    multiply along R), and x's column sums f32 [C], each if wanted, from one read.  tile 1: a scale per row's 128 elements; 128: per 128 x 128
+    tile, so that both forms hold the same values (weights).  include/w2c_hip.h w2c_quantize_fp8."""
+    if not x.is_cuda:
+        _need_gpu(x)
+    dev, code = x.device, _elem(x, "quantize_fp8")
+    if tile not in (1, FP8_BLOCK):
+        raise W2CError("quantize_fp8: tile is 1 or %d, got %r" % (FP8_BLOCK, tile))
+    if x.dim() != 2 or x.shape[1] < 1 or not (x.is_contiguous() or (x.stride(1) == 1 and x.stride(0) >= x.shape[1])):
+        raise W2CError("quantize_fp8: rows of at least one contiguous element expected, got %s with strides %s" % (tuple(x.shape), x.stride()))
+    if not (rows or columns or sums):
+        raise W2CError("quantize_fp8: nothing wanted")
+    R, C = x.shape
+    by_rows = _fp8_new(R, C, tile, dev) if rows else None
+    by_cols = _fp8_new(C, R, tile, dev) if columns else None
+    total = _empty((C,), torch.float32, dev) if sums else None
+    if not R:
+        if sums:
+            total.zero_()
+        return Fp8Quantized(by_rows, by_cols, total)
+    lib = _native.lib()
+    nbytes = lib.w2c_quantize_fp8_workspace_bytes(R, C) if sums else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if sums else None
+    with torch.cuda.device(dev):
+        check(lib.w2c_quantize_fp8(_p(x), code, R, C, x.stride(0) if R > 1 else C, tile, *((_p(by_rows.codes), _p(by_rows.scale)) if rows else (None, None)),
+                                   *((_p(by_cols.codes), _p(by_cols.scale)) if columns else (None, None)), _p(total), _p(ws), nbytes, _stream(dev)),
+              "w2c_quantize_fp8")
+    return Fp8Quantized(by_rows, by_cols, total)
+
+
+def _fp8_tile(t, what):
+    """rows that share a scale"""
+    codes, scale = t.codes, t.scale
+    if codes.dtype != torch.float8_e4m3fn or scale.dtype != torch.float8_e8m0fnu or codes.dim() != 2 or scale.dim() != 2:
+        raise W2CError("matmul_fp8: %s must be 2-D float8_e4m3fn codes with float8_e8m0fnu scales" % what)
+    R, K = codes.shape
+    if K % FP8_BLOCK or not 0 < t.cols <= K or scale.shape[1] * FP8_BLOCK != K or scale.shape[0] not in (R, -(-R // FP8_BLOCK)):
+        raise W2CError("matmul_fp8: %s: codes %s of %d columns with scales %s do not fit" % (what, tuple(codes.shape), t.cols, tuple(scale.shape)))
+    return 1 if scale.shape[0] == R else FP8_BLOCK
+
+
+def matmul_fp8(a, b, bias=None, out_dtype=BF16):
+    """a [M, K], b [N, K] (Fp8Blocks) -> a b^T (+ bias f32 [N]) as out_dtype [M, N]; f32 accumulation.  include/w2c_hip.h w2c_matmul_fp8."""
+    dev = _need_gpu(a.codes, a.scale, b.codes, b.scale, bias)
+    ta, tb = _fp8_tile(a, "a"), _fp8_tile(b, "b")
+    (M, K), (N, Kb) = a.codes.shape, b.codes.shape
+    if K != Kb or a.cols != b.cols:
+        raise W2CError("matmul_fp8: %d against %d columns" % (a.cols, b.cols))
+    if out_dtype not in _ELEM:
+        raise W2CError("matmul_fp8: f32, bf16 or f16 output expected, got %s" % out_dtype)
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,)):
+        raise W2CError("matmul_fp8: bias must be f32 [%d]" % N)
+    c = _empty((M, N), out_dtype, dev)
+    if M and N:
+        with torch.cuda.device(dev):
+            check(_native.lib().w2c_matmul_fp8(_p(a.codes), _p(a.scale), ta, _p(b.codes), _p(b.scale), tb, M, N, K, _p(bias), _p(c), _ELEM[out_dtype],
+                                               _stream(dev)), "w2c_matmul_fp8")
+    return c

@@ -388,6 +388,65 @@ class LayerNormHip(nn.LayerNorm):
         return layer_norm(x, self.weight, self.bias, self.eps, residual)
 
 
+class _LinearFp8Fn(torch.autograd.Function):
+    """y = x W^T + b with all three products of the training step in 8 bits (ops.matmul_fp8): x and dy with a scale per row's 128 elements of whatever
+    is summed over, W with a scale per 128 x 128 tile.  Every operand is read once and quantised both ways from that read."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        rows = x.reshape(-1, x.shape[-1])
+        xq = ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous(), 1, columns=need_w)
+        wq = ops.quantize_fp8(weight.detach().contiguous(), ops.FP8_BLOCK, columns=need_x)
+        y = ops.matmul_fp8(xq.rows, wq.rows, None if bias is None else bias.detach().float().contiguous(), x.dtype)
+        ctx.x_columns, ctx.w_columns = xq.columns, wq.columns
+        ctx.shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        return y.view(x.shape[:-1] + (weight.shape[0],))
+
+    @staticmethod
+    def backward(ctx, dy):
+        need_x, need_w, need_b = ctx.needs_input_grad
+        rows = dy.reshape(-1, dy.shape[-1])
+        q = ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous(), 1, rows=need_x, columns=need_w, sums=need_b)
+        dx = dw = db = None
+        if need_x:
+            dx = ops.matmul_fp8(q.rows, ctx.w_columns, None, ctx.dtypes[0]).view(ctx.shape)
+        if need_w:
+            if rows.shape[0]:
+                dw = ops.matmul_fp8(q.columns, ctx.x_columns, None, ctx.dtypes[1])
+            else:
+                dw = torch.zeros((dy.shape[-1], ctx.shape[-1]), dtype=ctx.dtypes[1], device=dy.device)
+        if need_b:
+            db = q.sums.to(ctx.dtypes[2])
+        return dx, dw, db
+
+
+def linear_fp8(x, weight, bias=None):
+    """y [..., N] = x [..., K] W^T + bias with the product (and, under autograd, both products of its backward) in 8 bits with a power-of-two scale
+    per 128 elements of the sum.  weight: [N, K] f32 / bf16 / f16, or ops.Fp8Blocks of it (quantize_fp8(weight, 128).rows: laid out once, for
+    inference).  HIP kernels under the "hip" backend on GPU tensors, F.linear otherwise."""
+    if isinstance(weight, ops.Fp8Blocks):
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ops.W2CError("linear_fp8: quantised weights are for inference; pass the weights themselves to differentiate")
+        if x.shape[-1] != weight.cols:
+            raise ops.W2CError("linear_fp8: %d features against weights of %d" % (x.shape[-1], weight.cols))
+        rows = x.reshape(-1, x.shape[-1])
+        y = ops.matmul_fp8(ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous()).rows, weight, bias, x.dtype)
+        return y.view(x.shape[:-1] + (y.shape[1],))
+    if _backend == "hip" and x.is_cuda:
+        if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or (bias is not None and tuple(bias.shape) != (weight.shape[0],)):
+            raise ops.W2CError("linear_fp8: x %s, weight %s and bias do not fit" % (tuple(x.shape), tuple(weight.shape)))
+        return _LinearFp8Fn.apply(x, weight, bias)
+    return F.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
+
+
+class LinearFp8(nn.Linear):
+    """nn.Linear (same parameters, same state_dict keys) on linear_fp8()"""
+
+    def forward(self, x):
+        return linear_fp8(x, self.weight, self.bias)
+
+
 class GraphedTrainStep:
     """One whole training step -- forward, loss, backward, optimizer step -- captured into ONE HIP graph and replayed (round 4
     item 9: the eager step is ~650 launches and host-bound).  Every kernel of the step is a stream operation (the HIP convs / BatchNorm /
