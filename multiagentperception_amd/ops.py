@@ -5,7 +5,11 @@ hands raw device pointers + sizes to libw2c_hip.so on torch's CURRENT stream of
 the tensor's device (so the path is re-entrant under DataParallel replicas and
 capturable in a graph).  There is no fallback: CPU tensors raise.
 """
-import ctypes
+import array
+import contextlib
+import functools
+import itertools
+import operator
 import threading
 import typing
 
@@ -37,7 +41,8 @@ def _stream(dev):
     rec = getattr(_tls, "recorder", None)
     if rec is not None:
         rec.dirty = True                            # this capture window holds at least one kernel node (ops.record_program)
-    return torch.cuda.current_stream(dev).cuda_stream
+    # (the raw handle: 0.1 us, a torch.cuda.Stream object around it 1.9)
+    return torch._C._cuda_getCurrentRawStream(dev.index if dev.index is not None else torch.cuda.current_device())
 
 
 def _p(t):
@@ -1779,6 +1784,14 @@ def nhwc_bf16_to_nchw_f32(x, channels=None):
 
 # ---- a model's head and its training step -----------------------------------------------------------------------------------------------
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev):
+    """the device to launch on; where it is the current one already (nearly always) this costs nothing"""
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
 _ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # the C ABI's element types
 
 
@@ -1812,11 +1825,12 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None):
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise W2CError("layer_norm: residual must have x's shape and type")
     rows = x.numel() // cols
-    y = _empty(x.shape, x.dtype, dev)
-    h = _empty(x.shape, x.dtype, dev) if residual is not None else x
-    mean, rstd = _empty(x.shape[:-1], torch.float32, dev), _empty(x.shape[:-1], torch.float32, dev)
+    y = torch.empty_like(x)
+    h = torch.empty_like(x) if residual is not None else x
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    rstd = torch.empty_like(mean)
     if rows:
-        with torch.cuda.device(dev):
+        with _on(dev):
             check(_native.lib().w2c_layer_norm_forward(_p(x), _p(residual), code, rows, cols, _p(weight), _p(bias), _ELEM[wtype], float(eps),
                                                        _p(y), _p(h) if residual is not None else None, _p(mean), _p(rstd), _stream(dev)),
                   "w2c_layer_norm_forward")
@@ -1850,7 +1864,7 @@ def layer_norm_backward(dy, h, weight, mean, rstd, dh=None, bias=True):
         if nbytes < 0:
             raise W2CError("layer_norm backward: %d rows of %d are out of range" % (rows, cols))
         ws = torch.empty(nbytes // 4, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(lib.w2c_layer_norm_backward(_p(dy), _p(h), _p(dh), code, rows, cols, _p(weight), _ELEM[wtype], _p(mean), _p(rstd), _p(dx), _p(dw),
                                           _p(db), _p(ws), nbytes, _stream(dev)), "w2c_layer_norm_backward")
     return dx, dw, db
@@ -1911,17 +1925,18 @@ def log_probs_forward(logits, target=None, top=0, dim=-1, ignore_index=-100):
         raise W2CError("log_probs: top must lie in 0 .. min(classes, %d), got %d of %d classes" % (LOG_PROBS_TOP_MOST, top, classes))
     if inner > 1 and classes > _LOG_PROBS_INNER_MOST:
         return log_probs_forward(logits.movedim(dim, -1).contiguous(), target, top, -1, ignore_index)
-    logp = _empty(rest, torch.float32, dev) if target is not None else None
-    entropy, stats = _empty(rest, torch.float32, dev), _empty(rest + (2,), torch.float32, dev)
-    top_logp = _empty(rest + (top,), torch.float32, dev) if top else None
-    top_index = _empty(rest + (top,), torch.int64, dev) if top else None
+    new = functools.partial(torch.empty, device=dev)
+    entropy, stats = new(rest, dtype=torch.float32), new(rest + (2,), dtype=torch.float32)
+    logp = torch.empty_like(entropy) if target is not None else None
+    top_logp = new(rest + (top,), dtype=torch.float32) if top else None
+    top_index = new(rest + (top,), dtype=torch.int64) if top else None
     if outer * inner:
         lib = _native.lib()
         nbytes = lib.w2c_log_probs_workspace_bytes(outer, classes, inner, top)
         if nbytes < 0:
             raise W2CError("log_probs: %d x %d x %d logits are out of range" % (outer, classes, inner))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with torch.cuda.device(dev):
+        with _on(dev):
             check(lib.w2c_log_probs_forward(_p(logits), code, outer, classes, inner, stride, _p(target), int(ignore_index), top, _p(logp), _p(entropy),
                                             _p(top_logp), _p(top_index), _p(stats), _p(ws), nbytes, _stream(dev)), "w2c_log_probs_forward")
     return LogProbs(logp, entropy, top_logp, top_index, stats)
@@ -1952,7 +1967,7 @@ def log_probs_backward(logits, target, forward, g_logp=None, g_entropy=None, g_t
         return d.movedim(-1, dim).contiguous()
     dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
     if outer * inner:
-        with torch.cuda.device(dev):
+        with _on(dev):
             check(_native.lib().w2c_log_probs_backward(_p(logits), code, outer, classes, inner, stride, _p(target), int(ignore_index),
                                                        _p(forward.stats), _p(forward.entropy), top, _p(forward.top_index), _p(g_logp),
                                                        _p(g_entropy), _p(g_top), _p(dx), _stream(dev)), "w2c_log_probs_backward")
@@ -1974,39 +1989,53 @@ def _dense(t):
     return True
 
 
-def _adamw_rows(params, grads, moments, steps):
-    """the C ABI's rows of nine int64 per tensor, after the checks that all four lists share"""
+_dtype, _device, _shape, _layout = (operator.attrgetter(n) for n in ("dtype", "device", "shape", "layout"))
+_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+
+
+def _rows(*columns):
+    """one int64 row of the C ABI per tensor from nine columns"""
+    return array.array("q", itertools.chain.from_iterable(zip(*columns)))
+
+
+def _adamw_tensors(params, grads):
+    """(device, addresses of the gradients, elements, element types) after the checks of parameters and gradients.  (Attribute by attribute over
+    whole lists: a step of a small network is bound by these checks.)"""
     n = len(params)
     if not n or len(grads) != n:
         raise W2CError("adamw: as many gradients as parameters expected, at least one (got %d and %d)" % (len(grads), n))
     dev = params[0].device
     if dev.type != "cuda":
         raise W2CError("w2c ops run only on an MI355X device tensor (got %s); there is no CPU fallback" % dev)
-    rows = []
-    for i, (p, g) in enumerate(zip(params, grads)):
-        code = _ELEM.get(p.dtype)
-        if code is None or g.dtype != p.dtype:
-            raise W2CError("adamw: parameter %d: f32, bf16 or f16 with a gradient of its type expected, got %s and %s" % (i, p.dtype, g.dtype))
-        if g.layout != torch.strided or g.shape != p.shape or g.device != dev or p.device != dev:
-            raise W2CError("adamw: parameter %d: a dense gradient of its shape on %s expected" % (i, dev))
-        if not (p.is_contiguous() and g.is_contiguous()) and (p.stride() != g.stride() or not _dense(p)):
-            raise W2CError("adamw: parameter %d and its gradient must be laid out alike, without gaps" % i)
-        m = moments[i] if moments is not None else (0, 0, 0, 0)
-        rows += (p.data_ptr(), g.data_ptr(), *m, steps[i] if steps is not None else 0, p.numel(), code)
-    return dev, (ctypes.c_longlong * len(rows))(*rows)
+    dtypes = list(map(_dtype, params))
+    if not set(dtypes) <= _ELEM.keys() or dtypes != list(map(_dtype, grads)):
+        raise W2CError("adamw: f32, bf16 or f16 parameters with gradients of their types expected")
+    if set(map(_layout, grads)) != {torch.strided} or list(map(_shape, params)) != list(map(_shape, grads)) or {dev} != {*map(_device, params), *map(_device, grads)}:
+        raise W2CError("adamw: dense gradients of the parameters' shapes on %s expected" % dev)
+    if not (all(map(_contiguous, params)) and all(map(_contiguous, grads))):
+        for i, (p, g) in enumerate(zip(params, grads)):
+            if not (p.is_contiguous() and g.is_contiguous()) and (p.stride() != g.stride() or not _dense(p)):
+                raise W2CError("adamw: parameter %d and its gradient must be laid out alike, without gaps" % i)
+    return dev, list(map(_ptr, grads)), list(map(_numel, params)), [_ELEM[d] for d in dtypes]
+
+
+def _grad_squares(dev, rows, n):
+    lib, at = _native.lib(), rows.buffer_info()[0]
+    count = lib.w2c_grad_squares_count(at, n)
+    if count < 0:
+        raise W2CError("grad_squares: a tensor is too large")
+    out = torch.empty(count, dtype=torch.float64, device=dev) if count else torch.zeros(1, dtype=torch.float64, device=dev)
+    if count:
+        with _on(dev):
+            check(lib.w2c_grad_squares(at, n, _p(out), count, _stream(dev)), "w2c_grad_squares")
+    return out
 
 
 def grad_squares(grads):
     """sums of the squares of parts of the gradients (f64), for adamw_step's `squares`: their total is the squared norm of all of them"""
-    dev, rows = _adamw_rows(grads, grads, None, None)
-    count = _native.lib().w2c_grad_squares_count(rows, len(grads))
-    if count < 0:
-        raise W2CError("grad_squares: a tensor is too large")
-    out = torch.zeros(1, dtype=torch.float64, device=dev) if count == 0 else torch.empty(count, dtype=torch.float64, device=dev)
-    if count:
-        with torch.cuda.device(dev):
-            check(_native.lib().w2c_grad_squares(rows, len(grads), _p(out), count, _stream(dev)), "w2c_grad_squares")
-    return out
+    dev, g, sizes, types = _adamw_tensors(grads, grads)
+    none = [0] * len(g)
+    return _grad_squares(dev, _rows(none, g, none, none, none, none, none, sizes, types), len(g))
 
 
 def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, max_norm=None, seed=0, squares=None):
@@ -2017,36 +2046,39 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
                                 scales of ADAMW_STATE_BLOCK elements; rounded at random by (seed, step, place)
     lr: a number, or an f32 device tensor of one element (a captured step then follows it).  max_norm: the gradients are scaled down to this
     norm in all; `squares` (grad_squares) where more tensors than these share the norm.  -> the norm before that (f32 on the device), or None."""
+    dev, g, sizes, types = _adamw_tensors(params, grads)
     n = len(params)
-    if len(states) != n or len(steps) != n:
-        raise W2CError("adamw: %d parameters, %d states, %d steps" % (n, len(states), len(steps)))
-    bits = 32 if n and len(states[0]) == 2 else 8
-    moments = []
-    for i, (p, st) in enumerate(zip(params, states)):
-        if len(st) != (2 if bits == 32 else 4) or any(t.device != p.device for t in st):
-            raise W2CError("adamw: the states must all be (m, v) or all (m, m_scale, v, v_scale), on the parameters' device")
-        k = p.numel()
-        if bits == 32:
-            m, v = st
-            for t in st:
-                if t.dtype != torch.float32 or t.numel() != k or not (p.is_contiguous() and t.is_contiguous() or t.stride() == p.stride()):
-                    raise W2CError("adamw: parameter %d: f32 moments laid out like it expected" % i)
-            moments.append((m.data_ptr(), v.data_ptr(), 0, 0))
-        else:
-            m, ms, v, vs = st
-            blocks = -(-k // ADAMW_STATE_BLOCK)
-            if (m.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or ms.dtype != torch.float8_e8m0fnu or vs.dtype != torch.float8_e8m0fnu
-                    or m.numel() != k or v.numel() != k or ms.numel() != blocks or vs.numel() != blocks
-                    or not (m.is_contiguous() and v.is_contiguous() and ms.is_contiguous() and vs.is_contiguous())):
-                raise W2CError("adamw: parameter %d: contiguous float8_e4m3fn moments of %d and float8_e8m0fnu scales of %d expected" % (i, k, blocks))
-            moments.append((m.data_ptr(), v.data_ptr(), ms.data_ptr(), vs.data_ptr()))
-    for i, t in enumerate(steps):
-        if t.dtype != torch.float32 or t.numel() != 1 or t.device != params[i].device:
-            raise W2CError("adamw: parameter %d: its step must be one f32 element on its device" % i)
-    counters = [t.data_ptr() for t in steps]
-    dev, rows = _adamw_rows(params, grads, moments, counters)
-    written = [rows[9 * i] for i in range(n) if rows[9 * i + 7]]
-    if len(set(written)) != len(written) or len(set(counters)) != n or len({a for m in moments for a in m if a}) != sum(1 for m in moments for a in m if a):
+    if len(states) != n or len(steps) != n or len({*map(len, states)}) != 1 or len(states[0]) not in (2, 4):
+        raise W2CError("adamw: a step and a state, all (m, v) or all (m, m_scale, v, v_scale), for each of %d parameters expected" % n)
+    bits = 32 if len(states[0]) == 2 else 8
+    parts = list(zip(*states))
+    for t in (*parts, steps):
+        if {*map(_device, t)} != {dev}:
+            raise W2CError("adamw: the states and steps must be on %s" % dev)
+    if bits == 32:
+        for t in parts:
+            if {*map(_dtype, t)} != {torch.float32} or list(map(_numel, t)) != sizes:
+                raise W2CError("adamw: f32 moments of the parameters' elements expected")
+            if not (all(map(_contiguous, t)) and all(map(_contiguous, params))):
+                for i, (p, q) in enumerate(zip(params, t)):
+                    if not (p.is_contiguous() and q.is_contiguous()) and p.stride() != q.stride():
+                        raise W2CError("adamw: parameter %d: its moments must be laid out like it" % i)
+        m, v = (list(map(_ptr, t)) for t in parts)
+        ms = vs = [0] * n
+        held = m + v
+    else:
+        blocks = [-(-k // ADAMW_STATE_BLOCK) for k in sizes]
+        for t, dtype, want in zip(parts, (torch.float8_e4m3fn, torch.float8_e8m0fnu) * 2, (sizes, blocks) * 2):
+            if {*map(_dtype, t)} != {dtype} or list(map(_numel, t)) != want or not all(map(_contiguous, t)):
+                raise W2CError("adamw: contiguous float8_e4m3fn moments of the parameters' elements and float8_e8m0fnu scales, one per %d of them, "
+                               "expected" % ADAMW_STATE_BLOCK)
+        m, ms, v, vs = (list(map(_ptr, t)) for t in parts)
+        held = m + ms + v + vs
+    if {*map(_dtype, steps)} != {torch.float32} or {*map(_numel, steps)} != {1}:
+        raise W2CError("adamw: steps must be one f32 element each")
+    counters = list(map(_ptr, steps))
+    written = [a for a in (*map(_ptr, params), *held, *counters) if a]          # (a tensor without elements has no address)
+    if len({*written}) != len(written):
         raise W2CError("adamw: a parameter, moment or step is in the lists twice")
     if max_norm is not None and not max_norm > 0:
         raise W2CError("adamw: max_norm must be positive, got %r" % (max_norm,))
@@ -2055,18 +2087,19 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
             raise W2CError("adamw: a tensor lr must be one f32 element on the parameters' device")
         lr_dev, lr = lr, 0.0
+    rows = _rows(map(_ptr, params), g, m, v, ms, vs, counters, sizes, types)
     norm = None
     if max_norm is not None:
         if squares is None:
-            squares = grad_squares(grads)
+            squares = _grad_squares(dev, rows, n)
         elif squares.dtype != torch.float64 or squares.device != dev or not squares.is_contiguous() or not squares.numel():
             raise W2CError("adamw: squares must come from grad_squares")
         norm = torch.empty((), dtype=torch.float32, device=dev)
     lib = _native.lib()
     nbytes = lib.w2c_adamw_workspace_bytes(n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        check(lib.w2c_adamw_step(rows, n, bits, float(lr), _p(lr_dev), float(beta1), float(beta2), float(eps), float(weight_decay),
+    with _on(dev):
+        check(lib.w2c_adamw_step(rows.buffer_info()[0], n, bits, float(lr), _p(lr_dev), float(beta1), float(beta2), float(eps), float(weight_decay),
                                  _p(squares) if norm is not None else None, squares.numel() if norm is not None else 0, float(max_norm or 0.0),
                                  _p(norm), int(seed) & 0xFFFFFFFF, _p(ws), nbytes, _stream(dev)), "w2c_adamw_step")
     torch.autograd.graph.increment_version(params)           # the engines' packed weights and autograd notice the in-place write
@@ -2091,8 +2124,8 @@ class Fp8Quantized(typing.NamedTuple):
 
 
 def _fp8_new(rows, cols, tile, dev):
-    codes = _empty((rows, -(-cols // FP8_BLOCK) * FP8_BLOCK), torch.float8_e4m3fn, dev)
-    return Fp8Blocks(codes, _empty((-(-rows // tile), codes.shape[1] // FP8_BLOCK), torch.float8_e8m0fnu, dev), cols)
+    codes = torch.empty((rows, -(-cols // FP8_BLOCK) * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=dev)
+    return Fp8Blocks(codes, torch.empty((-(-rows // tile), codes.shape[1] // FP8_BLOCK), dtype=torch.float8_e8m0fnu, device=dev), cols)
 
 
 def quantize_fp8(x, tile=1, rows=True, columns=False, sums=False):
@@ -2111,7 +2144,7 @@ def quantize_fp8(x, tile=1, rows=True, columns=False, sums=False):
     R, C = x.shape
     by_rows = _fp8_new(R, C, tile, dev) if rows else None
     by_cols = _fp8_new(C, R, tile, dev) if columns else None
-    total = _empty((C,), torch.float32, dev) if sums else None
+    total = torch.empty(C, dtype=torch.float32, device=dev) if sums else None
     if not R:
         if sums:
             total.zero_()
@@ -2119,7 +2152,7 @@ def quantize_fp8(x, tile=1, rows=True, columns=False, sums=False):
     lib = _native.lib()
     nbytes = lib.w2c_quantize_fp8_workspace_bytes(R, C) if sums else 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if sums else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(lib.w2c_quantize_fp8(_p(x), code, R, C, x.stride(0) if R > 1 else C, tile, *((_p(by_rows.codes), _p(by_rows.scale)) if rows else (None, None)),
                                    *((_p(by_cols.codes), _p(by_cols.scale)) if columns else (None, None)), _p(total), _p(ws), nbytes, _stream(dev)),
               "w2c_quantize_fp8")
@@ -2148,9 +2181,9 @@ def matmul_fp8(a, b, bias=None, out_dtype=BF16):
         raise W2CError("matmul_fp8: f32, bf16 or f16 output expected, got %s" % out_dtype)
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,)):
         raise W2CError("matmul_fp8: bias must be f32 [%d]" % N)
-    c = _empty((M, N), out_dtype, dev)
+    c = torch.empty((M, N), dtype=out_dtype, device=dev)
     if M and N:
-        with torch.cuda.device(dev):
+        with _on(dev):
             check(_native.lib().w2c_matmul_fp8(_p(a.codes), _p(a.scale), ta, _p(b.codes), _p(b.scale), tb, M, N, K, _p(bias), _p(c), _ELEM[out_dtype],
                                                _stream(dev)), "w2c_matmul_fp8")
     return c
