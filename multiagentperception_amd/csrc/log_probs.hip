@@ -77,13 +77,19 @@ __device__ __forceinline__ float key_value(key_t k) {
     const uint32_t o = (uint32_t)(k >> 32);
     return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ key_t max_key_step(key_t k) {
+    const key_t p = (key_t)dpp<CTRL, ROWS>(0u, (uint32_t)(k >> 32)) << 32 | dpp<CTRL, ROWS>(0u, (uint32_t)k);
+    return p > k ? p : k;
+}
 __device__ __forceinline__ key_t wave_max_key(key_t k) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const key_t p = __shfl_xor(k, o, 64);
-        k = p > k ? p : k;
-    }
-    return k;
+    k = max_key_step<0x111, 0xF>(k);
+    k = max_key_step<0x112, 0xF>(k);
+    k = max_key_step<0x114, 0xF>(k);
+    k = max_key_step<0x118, 0xF>(k);
+    k = max_key_step<0x142, 0xA>(k);
+    k = max_key_step<0x143, 0xC>(k);
+    return (key_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, 63);
 }
 
 struct Out {                                  // where a row's answers go
@@ -173,7 +179,7 @@ __global__ __launch_bounds__(256) void lp_lane_forward_kernel(const T* __restric
 // The top keys of NW waves' rows' parts, by rounds of the largest: `mine` is a lane's key; afterwards lane l < k of the FIRST wave holds the
 // l-th largest of the block's elements >= the bound.  lists: k * k keys, firsts: NW * k keys, both in shared memory.
 template <typename T, int NW>
-__device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int hi, int t, key_t mine, int k, key_t* lists, key_t* firsts, int* count) {
+__device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int hi, int first, key_t mine, int k, key_t* lists, key_t* firsts, int* count) {
     constexpr int VEC = ElemOf<T>::VEC, TPR = NW * 64;
     const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6;
     key_t left = mine, bound = 0;
@@ -204,12 +210,12 @@ __device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int h
     if (mine && mine >= bound) {                         // at most k threads
         key_t* list = lists + (long long)atomicAdd(count, 1) * k;
         int n = 0;
-        for (int c = lo + t * VEC; c < hi; c += TPR * VEC) {
+        for (int c = first; c < hi; c += TPR * VEC) {
             float v[VEC];
-            load_part<T, VEC>(p + c, hi - c, v);
+            load_range<T, VEC>(p, c, lo, hi, v, 0.f);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const key_t q = c + e < hi ? key_of(v[e], c + e) : 0;
+                const key_t q = c + e >= lo && c + e < hi ? key_of(v[e], c + e) : 0;
                 if (q >= bound && q && (n < k || q > list[n - 1])) {
                     int at = n < k ? n++ : n - 1;
                     for (; at > 0 && list[at - 1] < q; --at) list[at] = list[at - 1];
@@ -253,11 +259,10 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
     const T* p = x + row * row_stride;
     const int lo = blockIdx.y * part_len, hi = C - lo < part_len ? C : lo + part_len;
     Run r{-INFINITY, 0.f, 0.f};
+    const int first = lo - misaligned(p + lo) + t * VEC;
     float best = -INFINITY;
-    int at = lo + t * VEC;
-    for (int c = lo + t * VEC; c < hi; c += TPR * VEC) {
-        float v[VEC];
-        load_part<T, VEC>(p + c, hi - c, v, -INFINITY);
+    int at = first < lo ? lo : first;
+    auto take = [&](const float (&v)[VEC], int c) {
         const float cm = max_of<VEC>(v);
         if (k && cm > best) {
             best = cm;
@@ -266,6 +271,29 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
                 if (v[e] == cm) at = c + e;
         }
         run_add<VEC>(r, v, cm);
+    };
+    int c = first;
+    if (c < lo) {
+        float v[VEC];
+        load_range<T, VEC>(p, c, lo, hi, v, -INFINITY);
+        take(v, c);
+        c += TPR * VEC;
+    }
+    for (; c + 3 * TPR * VEC + VEC <= hi; c += 4 * TPR * VEC) {          // four accesses in flight per lane
+        u32x4_t raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = load_raw<T>(p + c + i * TPR * VEC);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v[VEC];
+            widen<T>(raw[i], v);
+            take(v, c + i * TPR * VEC);
+        }
+    }
+    for (; c < hi; c += TPR * VEC) {
+        float v[VEC];
+        load_range<T, VEC>(p, c, lo, hi, v, -INFINITY);
+        take(v, c);
     }
     r = wave_join(r);
     if constexpr (NW > 1) {
@@ -300,8 +328,8 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
     }
     if (!k) return;
     key_t* mem = shared + (NW == 1 ? wave * (k * k + 1) : 0);
-    const key_t mine = lo + t * VEC < hi ? key_of(best, at) : 0;
-    const key_t q = top_keys<T, NW>(p, lo, hi, t, mine, k, mem, mem + k * k, (int*)(mem + k * k + (NW == 1 ? 0 : NW * k)));
+    const key_t mine = first < hi ? key_of(best, at) : 0;
+    const key_t q = top_keys<T, NW>(p, lo, hi, first, mine, k, mem, mem + k * k, (int*)(mem + k * k + (NW == 1 ? 0 : NW * k)));
     if (wave == 0 || NW == 1) {
         s.m = __shfl(s.m, 0, 64);
         s.logs = __shfl(s.logs, 0, 64);
@@ -358,43 +386,58 @@ struct Grad {
     const long long* top_index;
     int top;
 };
+// dx_j = p_j (c1 l_j + c0) with l_j = log p_j, plus a at the target and b_i at the alternatives
 struct RowGrad {
-    float m, logs, H, a, whole, c;
-    long long t;
-    bool empty;
+    float m, logs, a, c0, c1;
+    int t;                                    // -1: none
 };
 __device__ __forceinline__ RowGrad row_grad(const Grad& g, long long row, int C) {
     RowGrad r;
     r.m = g.stats[2 * row];
     r.logs = g.stats[2 * row + 1];
-    r.H = g.entropy[row];
-    r.empty = r.logs == INFINITY;
     r.t = -1;
     r.a = 0.f;
     if (g.g_logp) {
         const long long t = g.target[row];
         if (t != g.ignore) {
-            r.t = t;
-            r.a = t < 0 || t >= C ? __builtin_nanf("") : g.g_logp[row];
+            const bool in = t >= 0 && t < C;
+            r.a = in ? g.g_logp[row] : __builtin_nanf("");
+            r.t = in ? (int)t : -1;
         }
     }
-    r.whole = r.a;
+    float whole = r.a;
     if (g.g_top)
-        for (int i = 0; i < g.top; ++i) r.whole += g.g_top[row * g.top + i];
-    r.c = g.g_entropy ? g.g_entropy[row] : 0.f;
+        for (int i = 0; i < g.top; ++i) whole += g.g_top[row * g.top + i];
+    const float c = g.g_entropy ? g.g_entropy[row] : 0.f;
+    r.c1 = -c;
+    r.c0 = -fmaf(c, g.entropy[row], whole);
+    if (r.logs == INFINITY) r.t = -1;         // a row of masked classes: p = 0 everywhere
     return r;
 }
-__device__ __forceinline__ float class_grad(const RowGrad& r, float x, int j) {
-    const float l = (x - r.m) - r.logs, p = exp_d(l);
-    float d = p == 0.f ? 0.f : -p * fmaf(r.c, l + r.H, r.whole);
-    if (j == r.t) d += r.a;
-    return r.empty ? 0.f : d;
+__device__ __forceinline__ float class_grad(const RowGrad& r, float x) {
+    const float l = (x - r.m) - r.logs;
+    return exp_d(l) * fmaf(r.c1, __builtin_fmaxf(l, LP_FLOOR), r.c0);
+}
+// the places that get more than that: lane 0 the target's, lane 1 + i the i-th alternative's (the same place: the same value)
+template <typename T>
+__device__ __forceinline__ void place_grad(const RowGrad& r, const Grad& g, long long row, int C, int lane, long long lo, long long hi, const T* p,
+                                           T* d, long long class_stride) {
+    const int top = g.g_top ? g.top : 0;
+    if (lane > top || r.logs == INFINITY) return;
+    const long long j = lane ? g.top_index[row * top + lane - 1] : r.t;
+    if (j < lo || j >= hi) return;
+    float v = class_grad(r, to_f32(p[j * class_stride])) + (j == r.t ? r.a : 0.f);
+    for (int i = 0; i < top; ++i)
+        if (g.top_index[row * top + i] == j) v += g.g_top[row * top + i];
+    d[j * class_stride] = from_f32<T>(v);
 }
 
-template <typename T>
+// KMAX alternatives in registers, their places compared with every class; KMAX = 0 with alternatives: those places are written again
+template <typename T, int KMAX>
 __global__ __launch_bounds__(256) void lp_lane_backward_kernel(const T* __restrict__ x, long long P, long long outer, int C, long long outer_stride,
                                                                long long row_stride, long long class_stride, Grad g, T* __restrict__ dx,
                                                                long long dx_outer_stride, long long dx_row_stride) {
+    constexpr int N = 8;
     const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= P) return;
     for (long long n = blockIdx.y; n < outer; n += gridDim.y) {
@@ -402,15 +445,33 @@ __global__ __launch_bounds__(256) void lp_lane_backward_kernel(const T* __restri
         const T* p = x + n * outer_stride + i * row_stride;
         T* d = dx + n * dx_outer_stride + i * dx_row_stride;
         const RowGrad r = row_grad(g, row, C);
-#pragma unroll 4
-        for (int j = 0; j < C; ++j) {
-            d[j * class_stride] = from_f32<T>(class_grad(r, to_f32(p[j * class_stride]), j));
+        float b[KMAX > 0 ? KMAX : 1];
+        int at[KMAX > 0 ? KMAX : 1];
+#pragma unroll
+        for (int k = 0; k < KMAX; ++k) {
+            const bool there = k < g.top && r.logs != INFINITY;
+            at[k] = there ? (int)g.top_index[row * g.top + k] : -1;
+            b[k] = there ? g.g_top[row * g.top + k] : 0.f;
         }
-        if (g.g_top && !r.empty)
-            for (int k = 0; k < g.top; ++k) {            // the alternatives' own terms: the same thread writes those places again
-                const long long j = g.top_index[row * g.top + k];
-                if (j >= 0 && j < C) d[j * class_stride] = from_f32<T>(class_grad(r, to_f32(p[j * class_stride]), (int)j) + g.g_top[row * g.top + k]);
-            }
+        for (int j = 0; j < C; j += N) {
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (j + e < C) v[e] = to_f32(p[(long long)(j + e) * class_stride]);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (j + e < C) {
+                    float w = class_grad(r, v[e]);
+                    if constexpr (KMAX > 0) {
+                        w += j + e == r.t ? r.a : 0.f;
+#pragma unroll
+                        for (int k = 0; k < KMAX; ++k) w += j + e == at[k] ? b[k] : 0.f;
+                    } else if (!g.g_top) w += j + e == r.t ? r.a : 0.f;
+                    d[(long long)(j + e) * class_stride] = from_f32<T>(w);
+                }
+        }
+        if (KMAX == 0 && g.g_top)
+            for (int k = 0; k <= g.top; ++k) place_grad<T>(r, g, row, C, k, 0, C, p, d, class_stride);
     }
 }
 
@@ -426,20 +487,38 @@ __global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restric
     T* d = dx + row * C;
     const int lo = blockIdx.y * part_len, hi = C - lo < part_len ? C : lo + part_len;
     const RowGrad r = row_grad(g, row, C);
-    for (int c = lo + t * VEC; c < hi; c += TPR * VEC) {
-        float v[VEC];
-        load_part<T, VEC>(p + c, hi - c, v);
+    auto take = [&](float (&v)[VEC]) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = class_grad(r, v[e], c + e);
-        store_part<T, VEC>(d + c, hi - c, v);
+        for (int e = 0; e < VEC; ++e) v[e] = class_grad(r, v[e]);
+    };
+    auto edge = [&](int c) {
+        float v[VEC];
+        load_range<T, VEC>(p, c, lo, hi, v, 0.f);
+        take(v);
+        store_range<T, VEC>(d, c, lo, hi, v);
+    };
+    int c = lo - misaligned(p + lo) + t * VEC;
+    if (c < lo) {
+        edge(c);
+        c += TPR * VEC;
     }
-    if (!g.g_top || r.empty) return;
+    for (; c + 3 * TPR * VEC + VEC <= hi; c += 4 * TPR * VEC) {          // four accesses in flight per lane
+        u32x4_t raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = load_raw<T>(p + c + i * TPR * VEC);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v[VEC];
+            widen<T>(raw[i], v);
+            take(v);
+            store_n<T, VEC>(d + c + i * TPR * VEC, v);
+        }
+    }
+    for (; c < hi; c += TPR * VEC) edge(c);
+    // (behind the block's stores to these places)
     if constexpr (NW > 1) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-    if (t < g.top) {
-        const long long j = g.top_index[row * g.top + t];
-        if (j >= lo && j < hi) d[j] = from_f32<T>(class_grad(r, to_f32(p[j]), (int)j) + g.g_top[row * g.top + t]);
-    }
+    place_grad<T>(r, g, row, C, t, lo, hi, p, d, 1);
 }
 
 // few long rows: enough parts for about four blocks on every CU, none under 256 lanes' accesses of 16 bytes
@@ -504,8 +583,13 @@ template <typename T>
 int lp_backward(const void* x, long long outer, int C, long long inner, long long row_stride, const Grad& g, void* dx, hipStream_t st) {
     if (lp_lane(C, inner)) {
         const LaneGrid l = lane_grid(outer, C, inner, row_stride);
-        hipLaunchKernelGGL((lp_lane_backward_kernel<T>), l.grid, l.block, 0, st, (const T*)x, l.P, l.outer, C, l.outer_stride, l.row_stride,
-                           l.class_stride, g, (T*)dx, l.outer_stride, inner > 1 ? 1ll : (long long)C);
+#define LP_LANE(K)                                                                                                                                \
+    hipLaunchKernelGGL((lp_lane_backward_kernel<T, K>), l.grid, l.block, 0, st, (const T*)x, l.P, l.outer, C, l.outer_stride, l.row_stride,          \
+                       l.class_stride, g, (T*)dx, l.outer_stride, inner > 1 ? 1ll : (long long)C)
+        if (!g.g_top || g.top > 8) LP_LANE(0);
+        else if (g.top <= 2) LP_LANE(2);
+        else LP_LANE(8);
+#undef LP_LANE
         return w2c_launch_status();
     }
     if (C <= LP_WAVE_MOST) {
@@ -513,7 +597,11 @@ int lp_backward(const void* x, long long outer, int C, long long inner, long lon
                            (T*)dx);
         return w2c_launch_status();
     }
-    const int len = 256 * ElemOf<T>::VEC * 8;              // eight accesses per lane
+    // a block per row, or per part of one where there are not rows enough for two rounds of blocks; at least four accesses per lane
+    long long n = (4096 + outer - 1) / outer;
+    const long long most = (C + 256 * ElemOf<T>::VEC * 4 - 1) / (256 * ElemOf<T>::VEC * 4);
+    if (n > most) n = most;
+    const int len = lp_part_len(C, (int)n);
     hipLaunchKernelGGL((lp_row_backward_kernel<T, 4>), dim3((unsigned)outer, (C - 1) / len + 1), dim3(256), 0, st, (const T*)x, outer, C, row_stride,
                        len, g, (T*)dx);
     return w2c_launch_status();
