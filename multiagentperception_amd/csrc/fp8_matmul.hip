@@ -12,7 +12,7 @@
 // but not below an f32 one's.  An f32 output therefore goes through the bf16 instructions, which keep 23: a code times its scale is a bf16
 // number exactly (one conversion instruction per pair does both), at half the rate.
 //
-//   tile kernels   at least 65 rows: TM x TN tiles, both operands by LDS-DMA into two stages of 128 k, one barrier per stage
+//   tile kernels   at least 65 rows: TM x TN tiles, both operands by LDS-DMA into a ring of four stages of 64 k
 //   row kernel     up to 64 rows (tokens being decoded): bound by reading b once; no LDS for operands, the waves of a block split k
 #include "lm_common.h"
 
@@ -58,13 +58,32 @@ __device__ __forceinline__ bf16x8_t scaled8(uint32_t lo, uint32_t hi, float s) {
     return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Stage image: row r (128 bytes) at r * 128, its 16-byte chunk c in slot c ^ ((r >> 1) & 7): 16 neighbouring rows' same chunk then cover all 64
-// banks once.  A piece of LDS-DMA is 8 rows (64 lanes x 16 bytes, contiguous in LDS); the swizzle is in the source address.
+__device__ __forceinline__ void dma4(unsigned dst, unsigned voff, u32x4_t srd, unsigned soff) {       // a dword per lane
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(srd), "s"(soff) : "memory", "m0");
+}
+__device__ __forceinline__ void dma1(unsigned dst, unsigned voff, u32x4_t srd, unsigned soff) {       // a byte per lane, into a dword of LDS
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ubyte %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(srd), "s"(soff) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_pieces() {               // at most N of this wave's LDS-DMA pieces are still under way; its LDS reads are done
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A ring of four stages of 64 k.  Step t multiplies stage t, whose operands are in registers already, reads stage t + 1's from LDS and sends for stage
+// t + 4, into the buffer of stage t (its reads were done before the barrier at the top of step t).  So a stage has three steps to arrive, and neither
+// its arrival nor an LDS read stands between the matrix instructions of two steps.  The scales of a block of 128 come with its first stage, into a
+// dword of LDS per row: four blocks' together where rows of scales are whole dwords (every row is a cache line of its own to the address unit:
+// 8192^3 to bf16 523 us with a byte per block, 512 with a dword per four; f32 outputs, at half the rate, lose 4 % by the branch and do without).
+// Stage image: row r (64 bytes) at 64 r, its 16-byte chunk c in slot c ^ ((r >> 2) & 3): 16 neighbouring rows' same chunk then cover all 64 banks once.
+// A piece of LDS-DMA is 16 rows (64 lanes x 16 bytes, contiguous in LDS); the swizzle is in the source address.
 template <typename T, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p, int tiles_m, int tiles_n) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int NW = WM * WN, MI = TM / WM / 32, NI = TN / WN / 32, PA = TM / 8 / NW, PB = TN / 8 / NW;
-    constexpr unsigned STAGE = (TM + TN) * KT;
+    constexpr int NW = WM * WN, MI = TM / WM / 32, NI = TN / WN / 32, PA = TM / 16 / NW, PB = TN / 16 / NW, HALF = KT / 2;
+    constexpr int PS = (TM + TN) / 64 / NW;                   // pieces of 64 rows of scales
+    constexpr unsigned STAGE = (TM + TN) * HALF, SCALES = 4 * STAGE, SBUF = (TM + TN) * 4;
     extern __shared__ __attribute__((aligned(1024))) u8 smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, lhi = lane >> 5;
     // tiles in groups of 8 tile rows, walked column by column: the 32 tiles in flight on an XCD share 8 row panels and 4 column panels
@@ -75,34 +94,66 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
         m0 = (8 * g + r % rows) * TM;
         n0 = (r / rows) * TN;
     }
-    const int ml = p.M - m0 < TM ? p.M - m0 : TM, nl = p.N - n0 < TN ? p.N - n0 : TN, KB = p.K / KT;
+    const int ml = p.M - m0 < TM ? p.M - m0 : TM, nl = p.N - n0 < TN ? p.N - n0 : TN, KB = p.K / KT, steps = 2 * KB;
     const u32x4_t srd_a = descriptor(p.a + (long long)m0 * p.K, (unsigned)ml * (unsigned)p.K);
     const u32x4_t srd_b = descriptor(p.b + (long long)n0 * p.K, (unsigned)nl * (unsigned)p.K);
     const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)W2C_LPTR(smem));
-    const int prow = wave * 8 + (lane >> 3), pchunk = (lane & 7) ^ ((prow >> 1) & 7);
-    const unsigned voff = (unsigned)prow * (unsigned)p.K + (unsigned)pchunk * 16u, vstep = (unsigned)(NW * 8) * (unsigned)p.K;
-    auto stage = [&](int kb) {
-        const unsigned dst = lds + (unsigned)(kb & 1) * STAGE + (unsigned)wave * 1024u, soff = (unsigned)kb * KT;
+    const int prow = wave * 16 + (lane >> 2), pchunk = (lane & 3) ^ ((lane >> 4) & 3);
+    const unsigned voff = (unsigned)prow * (unsigned)p.K + (unsigned)pchunk * 16u, vstep = (unsigned)(NW * 16) * (unsigned)p.K;
+    u32x4_t srd_s[PS];
+    unsigned svoff[PS];
 #pragma unroll
-        for (int i = 0; i < PA; ++i) dma16(dst + i * NW * 1024u, voff + i * vstep, srd_a, soff);
-#pragma unroll
-        for (int i = 0; i < PB; ++i) dma16(dst + TM * KT + i * NW * 1024u, voff + i * vstep, srd_b, soff);
+    for (int i = 0; i < PS; ++i) {                            // a piece's 64 rows are rows of a or of b; rows past the last repeat it
+        const int q = wave + NW * i;
+        const bool of_a = q < TM / 64;
+        const int row = (of_a ? m0 : n0 - TM) + q * 64 + lane, last = (of_a ? p.M : p.N) - 1, shift = of_a ? p.a_shift : p.b_shift;
+        const int first = (of_a ? m0 : n0) >> shift, count = (last >> shift) + 1 - first;
+        srd_s[i] = descriptor((of_a ? p.sa : p.sb) + (long long)first * KB, (unsigned)(count < TM + TN ? count : TM + TN) * (unsigned)KB);
+        svoff[i] = (unsigned)(((row < last ? row : last) >> shift) - first) * (unsigned)KB;
+    }
+    const bool packed = sizeof(T) == 2 && (KB & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.sa) | reinterpret_cast<uintptr_t>(p.sb)) & 3) == 0;
+    // piece i of stage t: scales first (a stage pair's come with its even one), then a's rows, then b's.  Behind the last stage the last is sent
+    // again, into buffers that nothing reads any more: every step then has the same pieces to wait for.
+    auto send = [&](int t, int i, bool with_scales) {
+        const int u = t < steps ? t : steps - 1;
+        const unsigned dst = lds + (unsigned)(t & 3) * STAGE + (unsigned)wave * 1024u, soff = (unsigned)u * HALF;
+        if (with_scales) {
+            if (i < PS) {
+                const unsigned to = lds + SCALES + (unsigned)(wave + NW * i) * 256u;
+                if (!packed) dma1(to + (unsigned)((t >> 1) & 1) * SBUF, svoff[i], srd_s[i], (unsigned)(u >> 1));
+                else if (!(t & 7)) dma4(to + (unsigned)((t >> 3) & 1) * SBUF, svoff[i], srd_s[i], (unsigned)(u >> 1) & ~3u);
+                return;
+            }
+            i -= PS;
+        }
+        if (i < PA) dma16(dst + i * NW * 1024u, voff + i * vstep, srd_a, soff);
+        else dma16(dst + TM * HALF + (i - PA) * NW * 1024u, voff + (i - PA) * vstep, srd_b, soff);
     };
+    constexpr int EACH = PA + PB, TWO = 2 * EACH + (sizeof(T) == 4 ? PS : 0);      // pieces of a stage, and what two neighbours have at least
     const int wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
-    const u8 *psa[MI], *psb[NI];
-    int sa[MI], sb[NI], sa_next[MI], sb_next[NI];
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        const int r = m0 + wm + i * 32 + l31;
-        psa[i] = p.sa + (long long)((r < p.M ? r : p.M - 1) >> p.a_shift) * KB;
-        sa_next[i] = *psa[i];
-    }
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-        const int r = n0 + wn + j * 32 + l31;
-        psb[j] = p.sb + (long long)((r < p.N ? r : p.N - 1) >> p.b_shift) * KB;
-        sb_next[j] = *psb[j];
-    }
+    // a lane's 32 bytes of a stage: chunks 2 lhi, 2 lhi + 1 of rows l31 of its fragments
+    const int key = (l31 >> 2) & 3, s0 = (((2 * lhi) ^ key) << 4), s1 = (((2 * lhi + 1) ^ key) << 4);
+    const u8* ra = smem + (wm + l31) * HALF;
+    const u8* rb = smem + (TM + wn + l31) * HALF;
+    struct Operands {
+        u32x4_t a[MI][2], b[NI][2];
+    };
+    constexpr int READS = 2 * (MI + NI), SREADS = MI + NI, MULTS = MI * NI;
+    auto read = [&](Operands& f, unsigned buf, int i) {       // one of READS: b's fragments first
+        const int k = i >> 1, h = i & 1;
+        if (k < NI) f.b[k][h] = *reinterpret_cast<const u32x4_t*>(rb + buf + (h ? s1 : s0) + k * 32 * HALF);
+        else f.a[k - NI][h] = *reinterpret_cast<const u32x4_t*>(ra + buf + (h ? s1 : s0) + (k - NI) * 32 * HALF);
+    };
+    struct Scales {
+        int a[MI], b[NI];
+    };
+    auto read_scales = [&](Scales& x, int kb, int i) {
+        const int* s = reinterpret_cast<const int*>(smem + SCALES + ((packed ? kb >> 2 : kb) & 1) * SBUF) + l31;
+        int v = s[i < NI ? TM + wn + i * 32 : wm + (i - NI) * 32] >> (packed ? 8 * (kb & 3) : 0);      // the scaled instructions take the lowest byte,
+        if constexpr (sizeof(T) == 4) v = (v & 255) << 23;                                             // the conversion a float's exponent field
+        if (i < NI) x.b[i] = v;
+        else x.a[i - NI] = v;
+    };
     f32x16_t acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -110,104 +161,91 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    // a lane's 32 bytes of k half h: chunks 4 h + 2 lhi, + 1
-    const int key = (l31 >> 1) & 7;
-    const u8* ra = smem + (wm + l31) * KT;
-    const u8* rb = smem + (TM + wn + l31) * KT;
-    int slot[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) slot[q] = ((((q >> 1) * 4 + 2 * lhi + (q & 1)) ^ key) << 4);
-    stage(0);
-    for (int kb = 0; kb < KB; ++kb) {
-        // this wave's pieces of stage kb have landed and its reads of stage kb - 1 are done; behind the barrier everyone's are
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        // the scales of this stage came with it; they are taken here, before the next stage's loads are issued, so that no wait for them
-        // can end up behind those
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            asm volatile("" : "+v"(sa_next[i]));
-            sa[i] = sa_next[i];
-        }
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            asm volatile("" : "+v"(sb_next[j]));
-            sb[j] = sb_next[j];
-        }
-        if (kb + 1 < KB) {
-            stage(kb + 1);
-#pragma unroll
-            for (int i = 0; i < MI; ++i) sa_next[i] = psa[i][kb + 1];
-#pragma unroll
-            for (int j = 0; j < NI; ++j) sb_next[j] = psb[j][kb + 1];
-        }
-        const unsigned buf = (unsigned)(kb & 1) * STAGE;
+    auto multiply = [&](const Operands& f, const Scales& x, int i, int j) {
         if constexpr (sizeof(T) == 4) {
-            float xa[MI], xb[NI];
 #pragma unroll
-            for (int i = 0; i < MI; ++i) xa[i] = __uint_as_float((uint32_t)sa[i] << 23);
-#pragma unroll
-            for (int j = 0; j < NI; ++j) xb[j] = __uint_as_float((uint32_t)sb[j] << 23);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                u32x4_t ca[MI], cb[NI];
-#pragma unroll
-                for (int j = 0; j < NI; ++j) cb[j] = *reinterpret_cast<const u32x4_t*>(rb + buf + j * 32 * KT + slot[q]);
-#pragma unroll
-                for (int i = 0; i < MI; ++i) ca[i] = *reinterpret_cast<const u32x4_t*>(ra + buf + i * 32 * KT + slot[q]);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    bf16x8_t fb[NI];
-#pragma unroll
-                    for (int j = 0; j < NI; ++j) fb[j] = scaled8(cb[j][2 * h], cb[j][2 * h + 1], xb[j]);
-#pragma unroll
-                    for (int i = 0; i < MI; ++i) {
-                        const bf16x8_t fa = scaled8(ca[i][2 * h], ca[i][2 * h + 1], xa[i]);
-#pragma unroll
-                        for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[j], fa, acc[i][j], 0, 0, 0);
-                    }
-                }
+            for (int q = 0; q < 4; ++q) {                     // 16 k each
+                const bf16x8_t fb = scaled8(f.b[j][q >> 1][2 * (q & 1)], f.b[j][q >> 1][2 * (q & 1) + 1], __int_as_float(x.b[j]));
+                const bf16x8_t fa = scaled8(f.a[i][q >> 1][2 * (q & 1)], f.a[i][q >> 1][2 * (q & 1) + 1], __int_as_float(x.a[i]));
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb, fa, acc[i][j], 0, 0, 0);
             }
-        } else {
+        } else
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat_i32x8(f.b[j][0], f.b[j][1]), cat_i32x8(f.a[i][0], f.a[i][1]), acc[i][j], 0, 0, 0,
+                                                                        x.b[j], 0, x.a[i]);
+    };
+    // step t: multiply `now`, read stage t + 1 into `next`, send stage t + 4.  Reads and pieces are spread between the matrix instructions: in one go they
+    // would hold up the only wave of the SIMD for as long as the LDS and the address unit take for all four waves' (8192^3 to bf16: 721 us against 603).
+    // What is left is bound by power: the same product of zeros takes 360 us, of random codes 515; matrix instructions alone reach 3.7 PFLOP/s on random codes.
+    auto step = [&](const Operands& now, Operands& next, const Scales& x, Scales& x_next, int t, bool second) {
+        const unsigned buf = (unsigned)((t + 1) & 3) * STAGE;
+        const int pieces = EACH + (second ? 0 : PS), reads = READS + (second ? SREADS : 0);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            i32x8_t fa[MI], fb[NI];
+        for (int m = 0; m < MULTS; ++m) {
 #pragma unroll
-            for (int j = 0; j < NI; ++j)
-                fb[j] = cat_i32x8(*reinterpret_cast<const u32x4_t*>(rb + buf + j * 32 * KT + slot[2 * h]),
-                                  *reinterpret_cast<const u32x4_t*>(rb + buf + j * 32 * KT + slot[2 * h + 1]));
+            for (int i = m * reads / MULTS; i < (m + 1) * reads / MULTS; ++i) {
+                if (i < READS) read(next, buf, i);
+                else read_scales(x_next, (t + 1) >> 1, i - READS);
+            }
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
-                fa[i] = cat_i32x8(*reinterpret_cast<const u32x4_t*>(ra + buf + i * 32 * KT + slot[2 * h]),
-                                  *reinterpret_cast<const u32x4_t*>(ra + buf + i * 32 * KT + slot[2 * h + 1]));
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j], fa[i], acc[i][j], 0, 0, 0, sb[j], 0, sa[i]);
+            for (int i = m * pieces / MULTS; i < (m + 1) * pieces / MULTS; ++i) send(t + 4, i, !second);
+            multiply(now, x, m / NI, m % NI);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        }
+    };
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < EACH + (t & 1 ? 0 : PS); ++i) send(t, i, !(t & 1));
+    wait_pieces<EACH + TWO>();
+    Operands even, odd;
+    Scales x, x_next;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) read(even, 0, i);
+#pragma unroll
+    for (int i = 0; i < SREADS; ++i) read_scales(x, 0, i);
+    for (int t = 0; t < steps; t += 2) {
+        wait_pieces<TWO>();                                   // stage t + 1 has landed everywhere
+        step(even, odd, x, x_next, t, false);
+        wait_pieces<TWO>();                                   // stage t + 2
+        step(odd, even, x, x_next, t + 1, true);
+        x = x_next;
     }
-    // accumulator e of a lane: column n = (e & 3) + 8 (e >> 2) + 4 lhi, row m = l31 of its 32 x 32 tile
+    // The accumulators of a fragment row (32 rows of the wave's part) go through LDS, f32, so that whole lines of c are written: stored as they lie,
+    // 8 bytes of each of 32 rows at a time, the epilogue took 28 us a tile.  Accumulator e of a lane: column (e & 3) + 8 (e >> 2) + 4 lhi, row l31 of its
+    // 32 x 32.  (The ring's last pieces are waited for: they may not land in this.)
+    wait_pieces<0>();
+    constexpr int COLS = TN / WN, PITCH = COLS + 4, VEC = ElemOf<T>::VEC, LANES = COLS / VEC, ROWS = 64 / LANES;
+    static_assert(NW * 32 * PITCH * 4 <= 4 * STAGE, "the epilogue fits the ring");
+    float* mine = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
+    const int col = lane % LANES * VEC, n = n0 + wn + col, left = p.N - n;
+    const bool whole = m0 + TM <= p.M && n0 + TN <= p.N;
+    float bias[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) bias[e] = p.bias && e < left ? p.bias[n + e] : 0.f;
     T* C = (T*)p.c;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-        const int m = m0 + wm + i * 32 + l31;
-        if (m >= p.M) continue;
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + wn + j * 32 + 8 * q + 4 * lhi, left = p.N - n;
-                float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                if (p.bias) {
-                    float bias[4];
-                    load_part<float, 4>(p.bias + n, left, bias);
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f32x4_t*>(mine + l31 * PITCH + j * 32 + 8 * q + 4 * lhi) =
+                    f32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // the wave's own: nobody else reads or writes them
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += bias[e];
-                }
-                store_part<T, 4>(C + (long long)m * p.N + n, left, v);
+        for (int r = 0; r < 32; r += ROWS) {
+            const int row = r + lane / LANES, m = m0 + wm + i * 32 + row;
+            float v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+                const f32x4_t w = *reinterpret_cast<const f32x4_t*>(mine + row * PITCH + col + e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[e + k] = w[k] + bias[e + k];
             }
+            if (whole) store_n<T, VEC>(C + (long long)m * p.N + n, v);
+            else if (m < p.M) store_part<T, VEC>(C + (long long)m * p.N + n, left, v);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 #endif
 }
@@ -430,7 +468,7 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
 template <typename T, int TM, int TN, int WM, int WN>
 int launch_tile(const Product& p, hipStream_t st) {
     const int tm = (p.M + TM - 1) / TM, tn = (p.N + TN - 1) / TN;
-    constexpr int lds = 2 * (TM + TN) * KT;
+    constexpr int lds = 4 * (TM + TN) * (KT / 2) + 2 * (TM + TN) * 4;
     static std::atomic<bool> big[64] = {};                    // per device: the kernel may use more than 64 KiB of LDS
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return w2c_launch_status();
@@ -454,7 +492,7 @@ int launch_product(const Product& p, hipStream_t st) {
         return w2c_launch_status();
     }
     // the large tile halves the traffic per product, but only where there are tiles for most of the 256 CUs
-    if ((long long)((p.M + 255) / 256) * ((p.N + 255) / 256) >= 160) return launch_tile<T, 256, 256, 2, 4>(p, st);
+    if ((long long)((p.M + 255) / 256) * ((p.N + 255) / 256) >= 160) return launch_tile<T, 256, 256, 2, 2>(p, st);
     return launch_tile<T, 128, 128, 2, 2>(p, st);
 }
 
