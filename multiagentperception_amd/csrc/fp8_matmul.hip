@@ -333,47 +333,71 @@ struct Quantize {
     u8 *codes, *scale, *codes_t, *scale_t;    // [rows][cp], [rows or tiles][cp / 128]; [cols][rp], [cols or tiles][rp / 128]; NULL: not wanted
     float* sums;                              // [tiles of rows][cols]
 };
+// The tile stays in registers between its read and its two ways out, and the column reductions share their LDS with the transposed image.
+// HBM-bound: 8192 x 4096 bf16 both ways, 134 MB, 32 us = 4.2 TB/s (36 with column sums); three blocks a CU by their registers.  Held to fewer
+// registers the compiler spills the tile (100 us).
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_kernel(Quantize q) {
-    constexpr int PITCH = 144;                                 // bytes of a column in the transposed image
-    __shared__ float col_amax[16][128];
-    __shared__ float col_sum[16][128];
-    __shared__ int col_e[128];
+    constexpr int PITCH = 136, VEC = ElemOf<T>::VEC, ACC = 8 / VEC;      // bytes of a column in the transposed image
+    union Shared {
+        struct {
+            float amax[16][128], sum[16][128];
+        } col;
+        u8 image[128 * PITCH];
+    };
+    __shared__ __attribute__((aligned(16))) Shared sh;
+    __shared__ float col_scale[128];
     __shared__ float tile_amax[4];
-    __shared__ __attribute__((aligned(16))) u8 image[128 * PITCH];
     const T* x = (const T*)q.x;
     const int tid = threadIdx.x, g = tid >> 4, l = tid & 15;   // rows 8 g .. + 7, columns 8 l .. + 7 of the tile
     const long long tr = blockIdx.y, tc = blockIdx.x, r0 = tr * 128 + g * 8, c0 = tc * 128 + l * 8;
     const long long kc = (q.cols + 127) / 128, kr = (q.rows + 127) / 128;
-    float v[8][8], ca[8], cs[8], ra[8];
+    u32x4_t raw[8][ACC];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const T* src = x + (r0 + i) * q.stride + c0;
+#pragma unroll
+        for (int k = 0; k < ACC; ++k) {
+            const long long left = r0 + i < q.rows ? q.cols - c0 - k * VEC : 0;
+            if (left >= VEC) raw[i][k] = load_raw<T>(src + k * VEC);
+            else {
+                Pack<T, VEC> t;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) t.v[e] = e < left ? src[k * VEC + e] : from_f32<T>(0.f);
+                raw[i][k] = __builtin_bit_cast(u32x4_t, t);
+            }
+        }
+    }
+    auto row_of = [&](int i, float (&v)[8]) {
+#pragma unroll
+        for (int k = 0; k < ACC; ++k) {
+            float w[VEC];
+            widen<T>(raw[i][k], w);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[k * VEC + e] = w[e];
+        }
+    };
+    const bool columns = q.codes_t || q.sums;
+    float ca[8], cs[8], ra[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) ca[e] = cs[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const long long left = r0 + i < q.rows ? q.cols - c0 : 0;
-        const T* src = x + (r0 + i) * q.stride + c0;
-        if constexpr (sizeof(T) == 4) {
-            float lo[4], hi[4];
-            load_part<T, 4>(src, left, lo);
-            load_part<T, 4>(src + 4, left - 4, hi);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[i][e] = lo[e];
-                v[i][4 + e] = hi[e];
-            }
-        } else load_part<T, 8>(src, left, v[i]);
-        float a = 0.f;
+        float v[8], a = 0.f;
+        row_of(i, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float m = __builtin_fabsf(v[i][e]) < INFINITY ? __builtin_fabsf(v[i][e]) : 0.f;      // of the finite values
+            const float m = __builtin_fabsf(v[e]) < INFINITY ? __builtin_fabsf(v[e]) : 0.f;            // of the finite values
             a = __builtin_fmaxf(a, m);
             ca[e] = __builtin_fmaxf(ca[e], m);
-            cs[e] += v[i][e];
+            cs[e] += v[e];
         }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) a = __builtin_fmaxf(a, __shfl_xor(a, o, 16));
         ra[i] = a;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) ra[i] = __builtin_fmaxf(ra[i], __shfl_xor(ra[i], o, 16));
     int e_tile = 0;
     if (q.tile == 128) {
         float a = ra[0];
@@ -388,63 +412,76 @@ __global__ __launch_bounds__(256) void quantize_kernel(Quantize q) {
             if (q.codes_t) q.scale_t[tc * kr + tr] = (u8)(e_tile + 127);
         }
     }
+    // no value is beyond 448 times its scale but infinities, and those and NaN become the NaN code
     if (q.codes) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (r0 + i >= q.rows) break;
             const int e = q.tile == 128 ? e_tile : scale_exponent(ra[i]);
             const float s = pow2f(-e);
-            uint32_t w[2] = {0, 0};
+            float v[8];
+            row_of(i, v);
+            uint32_t w[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {                     // no value is beyond 448 but infinities, and those and NaN become the NaN code
-                int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][4 * k] * s, v[i][4 * k + 1] * s, 0, false);
-                w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[i][4 * k + 2] * s, v[i][4 * k + 3] * s, t, true);
+            for (int k = 0; k < 2; ++k) {
+                const int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k] * s, v[4 * k + 1] * s, 0, false);
+                w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2] * s, v[4 * k + 3] * s, t, true);
             }
             __builtin_memcpy(q.codes + (r0 + i) * kc * 128 + c0, w, 8);
             if (q.tile == 1 && l == 0) q.scale[(r0 + i) * kc + tc] = (u8)(e + 127);
         }
     }
-    if (!q.codes_t && !q.sums) return;
+    if (!columns) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        col_amax[g][l * 8 + e] = ca[e];
-        col_sum[g][l * 8 + e] = cs[e];
+    for (int k = 0; k < 2; ++k) {
+        *reinterpret_cast<f32x4_t*>(&sh.col.amax[g][l * 8 + 4 * k]) = f32x4_t{ca[4 * k], ca[4 * k + 1], ca[4 * k + 2], ca[4 * k + 3]};
+        *reinterpret_cast<f32x4_t*>(&sh.col.sum[g][l * 8 + 4 * k]) = f32x4_t{cs[4 * k], cs[4 * k + 1], cs[4 * k + 2], cs[4 * k + 3]};
     }
     __syncthreads();
     if (tid < 128) {
         const long long c = tc * 128 + tid;
-        float a = col_amax[0][tid], s = col_sum[0][tid];
+        float a = sh.col.amax[0][tid];
 #pragma unroll
-        for (int k = 1; k < 16; ++k) {
-            a = __builtin_fmaxf(a, col_amax[k][tid]);
-            s += col_sum[k][tid];
-        }
-        col_e[tid] = q.tile == 128 ? e_tile : scale_exponent(a);
-        if (c < q.cols) {
-            if (q.sums) q.sums[tr * q.cols + c] = s;
-            if (q.codes_t && q.tile == 1) q.scale_t[c * kr + tr] = (u8)(col_e[tid] + 127);
-        }
+        for (int k = 1; k < 16; ++k) a = __builtin_fmaxf(a, sh.col.amax[k][tid]);
+        const int e = q.tile == 128 ? e_tile : scale_exponent(a);
+        col_scale[tid] = pow2f(-e);
+        if (c < q.cols && q.codes_t && q.tile == 1) q.scale_t[c * kr + tr] = (u8)(e + 127);
+    } else if (q.sums) {
+        const long long c = tc * 128 + tid - 128;
+        float s = sh.col.sum[0][tid - 128];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += sh.col.sum[k][tid - 128];
+        if (c < q.cols) q.sums[tr * q.cols + c] = s;
     }
     if (!q.codes_t) return;
-    __syncthreads();
+    __syncthreads();                                          // (the image overlays the reductions)
+    float s[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {                             // a column's eight rows are eight neighbouring bytes of the transposed image
-        const float s = pow2f(-col_e[l * 8 + e]);
-        uint32_t w[2];
+    for (int e = 0; e < 8; ++e) s[e] = col_scale[l * 8 + e];
+    uint32_t w[8][2];                                         // a column's eight rows are eight neighbouring bytes of the transposed image
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k][e] * s, v[4 * k + 1][e] * s, 0, false);
-            w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2][e] * s, v[4 * k + 3][e] * s, t, true);
-        }
-        *reinterpret_cast<uint64_t*>(image + (l * 8 + e) * PITCH + g * 8) = (uint64_t)w[1] << 32 | w[0];
+    for (int k = 0; k < 2; ++k) {
+        float v0[8], v1[8];
+        row_of(4 * k, v0);
+        row_of(4 * k + 1, v1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e][k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v0[e] * s[e], v1[e] * s[e], 0, false);
+        row_of(4 * k + 2, v0);
+        row_of(4 * k + 3, v1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e][k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v0[e] * s[e], v1[e] * s[e], (int)w[e][k], true);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) *reinterpret_cast<uint64_t*>(sh.image + (l * 8 + e) * PITCH + g * 8) = (uint64_t)w[e][1] << 32 | w[e][0];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {                             // 8 lanes write a column's 128 bytes
         const int cc = i * 32 + (tid >> 3), part = tid & 7;
         const long long c = tc * 128 + cc;
-        if (c < q.cols)
-            *reinterpret_cast<u32x4_t*>(q.codes_t + c * kr * 128 + tr * 128 + part * 16) = *reinterpret_cast<const u32x4_t*>(image + cc * PITCH + part * 16);
+        if (c < q.cols) {
+            const uint64_t lo = *reinterpret_cast<const uint64_t*>(sh.image + cc * PITCH + part * 16), hi = *reinterpret_cast<const uint64_t*>(sh.image + cc * PITCH + part * 16 + 8);
+            *reinterpret_cast<u32x4_t*>(q.codes_t + c * kr * 128 + tr * 128 + part * 16) = u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+        }
     }
 }
 
