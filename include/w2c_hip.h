@@ -554,9 +554,11 @@ int w2c_adamw_step(const long long* tensors, int n, int state_bits, double lr, c
 
 /* 8-bit product with a power-of-two scale per 128 of the reduction: c[m][n] = sum_k a[m][k] 2^(sa - 127) b[n][k] 2^(sb - 127) (+ bias[n]), c [M, N] of
  * dtype.  a [M, K], b [N, K]: e4m3fn codes, rows padded with zero codes to K, a multiple of 128, 16-byte aligned; a_scale e8m0
- * [a_tile = 1: M | 128: ceil(M / 128)][K / 128], b_scale alike: a scale per row or per 128 rows.  f32 accumulation, deterministic. */
+ * [a_tile = 1: M | 128: ceil(M / 128)][K / 128], b_scale alike: a scale per row or per 128 rows.  f32 accumulation, deterministic.  workspace: w2c_matmul_fp8_workspace_bytes
+ * (0: none), 16-byte aligned. */
+long long w2c_matmul_fp8_workspace_bytes(int M, int N, int K);
 int w2c_matmul_fp8(const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
-                   const float* bias, void* c, int dtype, w2c_stream_t stream);
+                   const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, w2c_stream_t stream);
 /* The codes and scales of x [rows, cols] (row stride `stride` elements): by rows (codes [rows, cols padded to 128], scale [rows, or ceil(rows / 128)
  * with tile 128][ceil(cols / 128)]), of the transposed x (codes_t [cols, rows padded to 128], 16-byte aligned, scale_t alike), either NULL if not
  * wanted, from one read.  A scale is the smallest power of two with amax <= 448 * scale, amax over the block's finite values (1 for zeros);

@@ -12,14 +12,17 @@
 // but not below an f32 one's.  An f32 output therefore goes through the bf16 instructions, which keep 23: a code times its scale is a bf16
 // number exactly (one conversion instruction per pair does both), at half the rate.
 //
-//   tile kernels   at least 65 rows: TM x TN tiles, both operands by LDS-DMA into a ring of four stages of 64 k
-//   row kernel     up to 64 rows (tokens being decoded): bound by reading b once; no LDS for operands, the waves of a block split k
+//   tile kernels   at least 25 rows: TM x TN tiles, both operands by LDS-DMA into a ring of four stages of 64 k
+//   row kernel     up to 24 rows (tokens being decoded): bound by reading b once; no LDS for operands, the waves of a block split k
 #include "lm_common.h"
 
 namespace {
 
 typedef unsigned char u8;
-constexpr int KT = 128;                       // elements of the reduction per scale, and per stage
+constexpr int KT = 128;                       // elements of the reduction per scale
+// The row kernel reads all of a once per 16 columns: against 16384 x 8192 weights it takes 27 us with 3 rows, 40 with 17, 46 with 24 and 52 with 32, the tile
+// kernels 42 to 46 with any of 17 to 64; against 1024 x 8192 it is 12 and 13 with 24 rows.
+constexpr int ROWS_MOST = 24;
 
 // four scale bytes (k blocks kb .. kb + 3) of a row; bytes past the row's end are not read, and not used
 __device__ __forceinline__ uint32_t scales4(const u8* p, int kb, int KB) {
@@ -38,6 +41,8 @@ struct Product {
     const float* bias;
     void* c;
     int M, N, K;                              // K: padded to 128
+    int parts;                                // > 1: the reduction is cut into that many parts of whole groups of four blocks (blockIdx.y)
+    float* part;                              // [parts][M][N] of them, added up by sum_splits_kernel
     int a_shift, b_shift;                     // row of the scales = row >> shift: 0 or 7
 };
 
@@ -82,7 +87,7 @@ template <typename T, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p, int tiles_m, int tiles_n) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int NW = WM * WN, MI = TM / WM / 32, NI = TN / WN / 32, PA = TM / 16 / NW, PB = TN / 16 / NW, HALF = KT / 2;
-    constexpr int PS = (TM + TN) / 64 / NW;                   // pieces of 64 rows of scales
+    constexpr int PS = ((TM + TN) / 64 + NW - 1) / NW;         // pieces of 64 rows of scales, at most, of a wave
     constexpr unsigned STAGE = (TM + TN) * HALF, SCALES = 4 * STAGE, SBUF = (TM + TN) * 4;
     extern __shared__ __attribute__((aligned(1024))) u8 smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, lhi = lane >> 5;
@@ -94,7 +99,9 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
         m0 = (8 * g + r % rows) * TM;
         n0 = (r / rows) * TN;
     }
-    const int ml = p.M - m0 < TM ? p.M - m0 : TM, nl = p.N - n0 < TN ? p.N - n0 : TN, KB = p.K / KT, steps = 2 * KB;
+    const int ml = p.M - m0 < TM ? p.M - m0 : TM, nl = p.N - n0 < TN ? p.N - n0 : TN, KB = p.K / KT;
+    const int k0 = p.parts > 1 ? (KB + 3) / 4 * (int)blockIdx.y / p.parts * 4 : 0;
+    const int k1 = p.parts > 1 && (int)blockIdx.y + 1 < p.parts ? (KB + 3) / 4 * ((int)blockIdx.y + 1) / p.parts * 4 : KB, steps = 2 * (k1 - k0);
     const u32x4_t srd_a = descriptor(p.a + (long long)m0 * p.K, (unsigned)ml * (unsigned)p.K);
     const u32x4_t srd_b = descriptor(p.b + (long long)n0 * p.K, (unsigned)nl * (unsigned)p.K);
     const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)W2C_LPTR(smem));
@@ -116,12 +123,14 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
     // again, into buffers that nothing reads any more: every step then has the same pieces to wait for.
     auto send = [&](int t, int i, bool with_scales) {
         const int u = t < steps ? t : steps - 1;
-        const unsigned dst = lds + (unsigned)(t & 3) * STAGE + (unsigned)wave * 1024u, soff = (unsigned)u * HALF;
+        const unsigned dst = lds + (unsigned)(t & 3) * STAGE + (unsigned)wave * 1024u, soff = (unsigned)(k0 * 2 + u) * HALF;
         if (with_scales) {
             if (i < PS) {
+                if constexpr ((TM + TN) / 64 % NW != 0)
+                    if (wave + NW * i >= (TM + TN) / 64) return;
                 const unsigned to = lds + SCALES + (unsigned)(wave + NW * i) * 256u;
-                if (!packed) dma1(to + (unsigned)((t >> 1) & 1) * SBUF, svoff[i], srd_s[i], (unsigned)(u >> 1));
-                else if (!(t & 7)) dma4(to + (unsigned)((t >> 3) & 1) * SBUF, svoff[i], srd_s[i], (unsigned)(u >> 1) & ~3u);
+                if (!packed) dma1(to + (unsigned)((t >> 1) & 1) * SBUF, svoff[i], srd_s[i], (unsigned)(k0 + (u >> 1)));
+                else if (!(t & 7)) dma4(to + (unsigned)((t >> 3) & 1) * SBUF, svoff[i], srd_s[i], (unsigned)(k0 + (u >> 1)) & ~3u);
                 return;
             }
             i -= PS;
@@ -129,7 +138,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
         if (i < PA) dma16(dst + i * NW * 1024u, voff + i * vstep, srd_a, soff);
         else dma16(dst + TM * HALF + (i - PA) * NW * 1024u, voff + (i - PA) * vstep, srd_b, soff);
     };
-    constexpr int EACH = PA + PB, TWO = 2 * EACH + (sizeof(T) == 4 ? PS : 0);      // pieces of a stage, and what two neighbours have at least
+    constexpr int EACH = PA + PB, TWO = 2 * EACH + (sizeof(T) == 4 ? (TM + TN) / 64 / NW : 0);      // pieces of a stage, and what two neighbours have at least
     const int wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
     // a lane's 32 bytes of a stage: chunks 2 lhi, 2 lhi + 1 of rows l31 of its fragments
     const int key = (l31 >> 2) & 3, s0 = (((2 * lhi) ^ key) << 4), s1 = (((2 * lhi + 1) ^ key) << 4);
@@ -138,7 +147,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
     struct Operands {
         u32x4_t a[MI][2], b[NI][2];
     };
-    constexpr int READS = 2 * (MI + NI), SREADS = MI + NI, MULTS = MI * NI;
+    constexpr int READS = 2 * (MI + NI), SREADS = MI + NI, QUARTERS = sizeof(T) == 4 ? 4 : 1, MULTS = MI * NI * QUARTERS;
     auto read = [&](Operands& f, unsigned buf, int i) {       // one of READS: b's fragments first
         const int k = i >> 1, h = i & 1;
         if (k < NI) f.b[k][h] = *reinterpret_cast<const u32x4_t*>(rb + buf + (h ? s1 : s0) + k * 32 * HALF);
@@ -161,14 +170,11 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    auto multiply = [&](const Operands& f, const Scales& x, int i, int j) {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {                     // 16 k each
-                const bf16x8_t fb = scaled8(f.b[j][q >> 1][2 * (q & 1)], f.b[j][q >> 1][2 * (q & 1) + 1], __int_as_float(x.b[j]));
-                const bf16x8_t fa = scaled8(f.a[i][q >> 1][2 * (q & 1)], f.a[i][q >> 1][2 * (q & 1) + 1], __int_as_float(x.a[i]));
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb, fa, acc[i][j], 0, 0, 0);
-            }
+    auto multiply = [&](const Operands& f, const Scales& x, int q, int i, int j) {
+        if constexpr (sizeof(T) == 4) {                       // 16 k: a quarter of the stage
+            const bf16x8_t fb = scaled8(f.b[j][q >> 1][2 * (q & 1)], f.b[j][q >> 1][2 * (q & 1) + 1], __int_as_float(x.b[j]));
+            const bf16x8_t fa = scaled8(f.a[i][q >> 1][2 * (q & 1)], f.a[i][q >> 1][2 * (q & 1) + 1], __int_as_float(x.a[i]));
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb, fa, acc[i][j], 0, 0, 0);
         } else
             acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat_i32x8(f.b[j][0], f.b[j][1]), cat_i32x8(f.a[i][0], f.a[i][1]), acc[i][j], 0, 0, 0,
                                                                         x.b[j], 0, x.a[i]);
@@ -180,7 +186,10 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
         const unsigned buf = (unsigned)((t + 1) & 3) * STAGE;
         const int pieces = EACH + (second ? 0 : PS), reads = READS + (second ? SREADS : 0);
 #pragma unroll
-        for (int m = 0; m < MULTS; ++m) {
+        for (int q = 0; q < QUARTERS; ++q)
+#pragma unroll
+        for (int ij = 0; ij < MI * NI; ++ij) {
+            const int m = q * MI * NI + ij;
 #pragma unroll
             for (int i = m * reads / MULTS; i < (m + 1) * reads / MULTS; ++i) {
                 if (i < READS) read(next, buf, i);
@@ -188,7 +197,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
             }
 #pragma unroll
             for (int i = m * pieces / MULTS; i < (m + 1) * pieces / MULTS; ++i) send(t + 4, i, !second);
-            multiply(now, x, m / NI, m % NI);
+            multiply(now, x, q, ij / NI, ij % NI);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -221,7 +230,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
     const bool whole = m0 + TM <= p.M && n0 + TN <= p.N;
     float bias[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) bias[e] = p.bias && e < left ? p.bias[n + e] : 0.f;
+    for (int e = 0; e < VEC; ++e) bias[e] = p.bias && p.parts == 1 && e < left ? p.bias[n + e] : 0.f;
     T* C = (T*)p.c;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -242,15 +251,41 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[e + k] = w[k] + bias[e + k];
             }
-            if (whole) store_n<T, VEC>(C + (long long)m * p.N + n, v);
-            else if (m < p.M) store_part<T, VEC>(C + (long long)m * p.N + n, left, v);
+            const long long at = (long long)m * p.N + n;
+            if (p.parts > 1) {
+                if (m < p.M) store_part<float, VEC>(p.part + (long long)blockIdx.y * p.M * p.N + at, left, v);
+            } else if (whole) store_n<T, VEC>(C + at, v);
+            else if (m < p.M) store_part<T, VEC>(C + at, left, v);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 #endif
 }
 
-// Up to 16 MT rows of a against 16 rows of b per block; wave w takes its share of the k blocks, the partial tiles are added in wave order.
+// c = the parts' sum, in part order, + bias; four columns of a row per thread
+template <typename T>
+__global__ __launch_bounds__(256) void sum_splits_kernel(Product p) {
+    const long long groups = (p.N + 3) / 4, i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= groups * p.M) return;
+    const long long m = i / groups;
+    const int n = (int)(i - m * groups) * 4, left = p.N - n;
+    const float* q = p.part + m * p.N + n;
+    float v[4], w[4];
+    load_part<float, 4>(q, left, v);
+    for (int k = 1; k < p.parts; ++k) {
+        load_part<float, 4>(q + (long long)k * p.M * p.N, left, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += w[e];
+    }
+    if (p.bias) {
+        load_part<float, 4>(p.bias + n, left, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += w[e];
+    }
+    store_part<T, 4>((T*)p.c + m * p.N + n, left, v);
+}
+
+// At most 16 MT rows of a against 16 rows of b per block; wave w takes its share of the k blocks, the partial tiles are added in wave order.
 template <typename T, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void matmul_rows_kernel(Product p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -515,34 +550,70 @@ int launch_tile(const Product& p, hipStream_t st) {
             return w2c_launch_status();
         big[dev].store(true, std::memory_order_release);
     }
-    hipLaunchKernelGGL((matmul_tile_kernel<T, TM, TN, WM, WN>), dim3(tm * tn), dim3(WM * WN * 64), lds, st, p, tm, tn);
+    hipLaunchKernelGGL((matmul_tile_kernel<T, TM, TN, WM, WN>), dim3(tm * tn, p.parts), dim3(WM * WN * 64), lds, st, p, tm, tn);
+    if (p.parts > 1)
+        hipLaunchKernelGGL((sum_splits_kernel<T>), dim3((unsigned)(((long long)((p.N + 3) / 4) * p.M + 255) / 256)), dim3(256), 0, st, p);
     return w2c_launch_status();
+}
+
+long long tiles(int M, int N, int tm, int tn) { return (long long)((M + tm - 1) / tm) * ((N + tn - 1) / tn); }
+// What a product of the tile kernels is cut into: the largest tiles of which there are enough for the 256 CUs (a larger tile reads less per product),
+// and where there are not enough of the smallest, parts of the reduction, of at least four blocks of 128 each.
+struct Cut {
+    int tm, tn, parts;
+};
+Cut product_cut(int M, int N, int K) {
+    if (tiles(M, N, 256, 256) >= 160) return {256, 256, 1};
+    if (tiles(M, N, 128, 128) >= 224) return {128, 128, 1};
+    const long long t = tiles(M, N, 128, 64);
+    long long parts = t >= 192 ? 1 : 512 / t;
+    const int most = (K / KT + 3) / 4;
+    if (parts > most) parts = most;
+    if (parts > 16) parts = 16;
+    return {128, 64, (int)parts};
 }
 
 template <typename T>
 int launch_product(const Product& p, hipStream_t st) {
-    if (p.M <= 64) {
+    if (p.M <= ROWS_MOST) {
         const dim3 grid((p.N + 15) / 16);
-        if (p.M <= 16) hipLaunchKernelGGL((matmul_rows_kernel<T, 1, 4>), grid, dim3(256), 0, st, p);
-        else if (p.M <= 32) hipLaunchKernelGGL((matmul_rows_kernel<T, 2, 4>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((matmul_rows_kernel<T, 4, 4>), grid, dim3(256), 0, st, p);
+        // 16 waves to a block where 4 would leave the card without enough of them
+        const bool few = p.N < 16 * 768 && p.K >= 16 * KT;
+#define MATMUL_ROWS(MT)                                                                                                             \
+    do {                                                                                                                            \
+        if (few) hipLaunchKernelGGL((matmul_rows_kernel<T, MT, 16>), grid, dim3(1024), 0, st, p);                                    \
+        else hipLaunchKernelGGL((matmul_rows_kernel<T, MT, 4>), grid, dim3(256), 0, st, p);                                          \
+    } while (0)
+        if (p.M <= 16) MATMUL_ROWS(1);
+        else MATMUL_ROWS(2);
+#undef MATMUL_ROWS
         return w2c_launch_status();
     }
-    // the large tile halves the traffic per product, but only where there are tiles for most of the 256 CUs
-    if ((long long)((p.M + 255) / 256) * ((p.N + 255) / 256) >= 160) return launch_tile<T, 256, 256, 2, 2>(p, st);
-    return launch_tile<T, 128, 128, 2, 2>(p, st);
+    const Cut cut = product_cut(p.M, p.N, p.K);
+    if (cut.tm == 256) return launch_tile<T, 256, 256, 2, 2>(p, st);
+    if (cut.tn == 128) return launch_tile<T, 128, 128, 2, 2>(p, st);
+    return launch_tile<T, 128, 64, 2, 2>(p, st);
 }
 
 }  // namespace
 
+extern "C" long long w2c_matmul_fp8_workspace_bytes(int M, int N, int K) {
+    if (M < 1 || N < 1 || K < KT || K % KT) return W2C_E_ARG;
+    const int parts = M <= ROWS_MOST ? 1 : product_cut(M, N, K).parts;
+    return parts > 1 ? (long long)parts * M * N * (long long)sizeof(float) : 0;
+}
+
 extern "C" int w2c_matmul_fp8(const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
-                              const float* bias, void* c, int dtype, void* stream) {
+                              const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, void* stream) {
     if (!a || !a_scale || !b || !b_scale || !c || M < 1 || N < 1 || K < KT || K % KT || K > (1 << 22) || dtype < W2C_F32 || dtype > W2C_F16) return W2C_E_ARG;
     if ((a_tile != 1 && a_tile != 128) || (b_tile != 1 && b_tile != 128) || (long long)M * N > (1ll << 40)) return W2C_E_ARG;
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) return W2C_E_ARG;
     if ((long long)((M + 127) / 128) * ((N + 127) / 128) > 0x7FFFFFFF) return W2C_E_ARG;
     w2c_clear_error();
-    const Product p{(const u8*)a, (const u8*)a_scale, (const u8*)b, (const u8*)b_scale, bias, c, M, N, K, a_tile == 128 ? 7 : 0, b_tile == 128 ? 7 : 0};
+    const long long need = w2c_matmul_fp8_workspace_bytes(M, N, K);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return W2C_E_ARG;
+    const Product p{(const u8*)a, (const u8*)a_scale, (const u8*)b, (const u8*)b_scale, bias, c, M, N, K,
+                    M <= ROWS_MOST ? 1 : product_cut(M, N, K).parts, (float*)workspace, a_tile == 128 ? 7 : 0, b_tile == 128 ? 7 : 0};
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == W2C_F32) return launch_product<float>(p, st);
     if (dtype == W2C_BF16) return launch_product<bf16_t>(p, st);

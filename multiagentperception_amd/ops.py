@@ -2183,7 +2183,10 @@ def matmul_fp8(a, b, bias=None, out_dtype=BF16):
         raise W2CError("matmul_fp8: bias must be f32 [%d]" % N)
     c = torch.empty((M, N), dtype=out_dtype, device=dev)
     if M and N:
+        lib = _native.lib()
+        nbytes = lib.w2c_matmul_fp8_workspace_bytes(M, N, K)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
         with _on(dev):
-            check(_native.lib().w2c_matmul_fp8(_p(a.codes), _p(a.scale), ta, _p(b.codes), _p(b.scale), tb, M, N, K, _p(bias), _p(c), _ELEM[out_dtype],
-                                               _stream(dev)), "w2c_matmul_fp8")
+            check(lib.w2c_matmul_fp8(_p(a.codes), _p(a.scale), ta, _p(b.codes), _p(b.scale), tb, M, N, K, _p(bias), _p(c), _ELEM[out_dtype],
+                                     _p(ws), nbytes, _stream(dev)), "w2c_matmul_fp8")
     return c
