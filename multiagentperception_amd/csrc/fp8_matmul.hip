@@ -394,13 +394,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(Quantize q) {
 #pragma unroll
         for (int k = 0; k < ACC; ++k) {
             const long long left = r0 + i < q.rows ? q.cols - c0 - k * VEC : 0;
-            if (left >= VEC) raw[i][k] = load_raw<T>(src + k * VEC);
-            else {
-                Pack<T, VEC> t;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) t.v[e] = e < left ? src[k * VEC + e] : from_f32<T>(0.f);
-                raw[i][k] = __builtin_bit_cast(u32x4_t, t);
-            }
+            raw[i][k] = load_raw_part<T>(src + k * VEC, left);
         }
     }
     auto row_of = [&](int i, float (&v)[8]) {

@@ -94,6 +94,16 @@ __device__ __forceinline__ u32x4_t load_raw(const T* __restrict__ p) {
     __builtin_memcpy(&t, p, sizeof(t));
     return __builtin_bit_cast(u32x4_t, t);
 }
+// ... of which only the first n elements exist; the absent ones are `fill`
+template <typename T>
+__device__ __forceinline__ u32x4_t load_raw_part(const T* __restrict__ p, long long n, float fill = 0.f) {
+    constexpr int VEC = ElemOf<T>::VEC;
+    if (n >= VEC) return load_raw<T>(p);
+    Pack<T, VEC> t;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t.v[i] = i < n ? p[i] : from_f32<T>(fill);
+    return __builtin_bit_cast(u32x4_t, t);
+}
 template <typename T>
 __device__ __forceinline__ void widen(u32x4_t r, float (&v)[ElemOf<T>::VEC]) {
     const Pack<T, ElemOf<T>::VEC> t = __builtin_bit_cast(Pack<T, ElemOf<T>::VEC>, r);
