@@ -126,97 +126,122 @@ __global__ __launch_bounds__(256) void adamw32_kernel(Table t, const Factors* __
     }
 }
 
-__device__ __forceinline__ uint32_t random_bits(uint32_t key, long long place) {
-    uint32_t x = (uint32_t)place * 0xA3D8F62Bu + (uint32_t)(place >> 32) * 0xC2B2AE35u + key;
+// the bits of a place: `x` = place * 0xA3D8F62B + (place >> 32) * 0xC2B2AE35 + key
+__device__ __forceinline__ uint32_t random_bits(uint32_t x) {
     x = (x ^ (x >> 15)) * 0xC58B3E95u;
     x = (x ^ (x >> 13)) * 0x9E3779B1u;
     return x ^ (x >> 16);
 }
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
-// |x| <= 448 to an e4m3 code.  x * 2^-120 puts e4m3's exponent and mantissa fields (subnormals too) into bits 20.. of the f32: 20 random bits
-// below them and a cut round up with the cut-off part's share of a step as the chance.
-__device__ __forceinline__ uint32_t code_of(float x, uint32_t noise20, uint32_t least) {
-    const float t = x * 0x1p-120f;
-    uint32_t c = ((__float_as_uint(t) & 0x7FFFFFFFu) + noise20) >> 20;
-    c = c > 126u ? 126u : c;
-    c = c < least ? least : c;
-    c |= (__float_as_uint(x) >> 24) & 0x80u;
-    return finite(x) ? c : 0x7Fu;
+// The e4m3 code of |x| <= 448 2^e, sign aside.  x * 2^(-e - 120) puts e4m3's exponent and mantissa fields (subnormals too) into bits 20.. of the f32: 20
+// random bits below them and a cut round up with the cut-off part's share of a step as the chance.
+__device__ __forceinline__ uint32_t code_of(float x, int e, uint32_t noise20) {
+    return ((__float_as_uint(__builtin_amdgcn_ldexpf(x, -120 - e)) & 0x7FFFFFFFu) + noise20) >> 20;
 }
 
+// one block of 256 of a tensor: WHOLE, or its last `left` (counted from this lane's first element)
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void adamw8_block(const Factors& f, const Rates& k, T* P, const T* G, uint8_t* M, uint8_t* V, uint8_t* ms, uint8_t* vs,
+                                             long long place, long long left, int lane) {
+    constexpr int VEC = 4;                                    // elements per lane
+    float p[VEC], g[VEC], m[VEC], r[VEC];
+    uint32_t mc = 0, vc = 0;
+    if constexpr (WHOLE) {
+        load_n<T, VEC>(P, p);
+        load_n<T, VEC>(G, g);
+        __builtin_memcpy(&mc, M, 4);
+        __builtin_memcpy(&vc, V, 4);
+    } else {
+        load_part<T, VEC>(P, left, p);
+        load_part<T, VEC>(G, left, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (j < left) {
+                mc |= (uint32_t)M[j] << (8 * j);
+                vc |= (uint32_t)V[j] << (8 * j);
+            }
+    }
+    const float sm = pow2f((int)*ms - 127), sv = pow2f((int)*vs - 127);
+    m[0] = __builtin_amdgcn_cvt_f32_fp8(mc, 0) * sm;
+    m[1] = __builtin_amdgcn_cvt_f32_fp8(mc, 1) * sm;
+    m[2] = __builtin_amdgcn_cvt_f32_fp8(mc, 2) * sm;
+    m[3] = __builtin_amdgcn_cvt_f32_fp8(mc, 3) * sm;
+    r[0] = __builtin_amdgcn_cvt_f32_fp8(vc, 0) * sv;
+    r[1] = __builtin_amdgcn_cvt_f32_fp8(vc, 1) * sv;
+    r[2] = __builtin_amdgcn_cvt_f32_fp8(vc, 2) * sv;
+    r[3] = __builtin_amdgcn_cvt_f32_fp8(vc, 3) * sv;
+    float am = 0.f, ar = 0.f, odd = 0.f;                      // odd: NaN where a value is not finite
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        float v = r[j] * r[j];
+        adamw_element(k, f, g[j], p[j], m[j], v, r[j]);
+        if (!WHOLE && j >= left) m[j] = r[j] = 0.f;
+        am = __builtin_fmaxf(am, __builtin_fabsf(m[j]));
+        ar = __builtin_fmaxf(ar, r[j]);
+        odd = fmaf(m[j], 0.f, fmaf(r[j], 0.f, odd));
+    }
+    if constexpr (WHOLE) store_n<T, VEC>(P, p);
+    else store_part<T, VEC>(P, left, p);
+    const bool any_odd = __any(odd != 0.f);                   // (NaN != 0)
+    if (any_odd) {                                            // rare: the scale comes from the finite values
+        am = ar = 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            if (finite(m[j])) am = __builtin_fmaxf(am, __builtin_fabsf(m[j]));
+            if (finite(r[j])) ar = __builtin_fmaxf(ar, r[j]);
+        }
+    }
+    const int em = scale_exponent(wave_max(am)), ev = scale_exponent(wave_max(ar));
+    const uint32_t seed = (uint32_t)place * 0xA3D8F62Bu + (uint32_t)(place >> 32) * 0xC2B2AE35u + f.key;
+    mc = vc = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        // (a block's places share their upper half: 256 divides 2^32)
+        const uint32_t x = random_bits(seed + (uint32_t)j * 0xA3D8F62Bu);
+        uint32_t cm = code_of(m[j], em, (x << 4 & 0xFFFF0u) + 8u) | (__float_as_uint(m[j]) >> 24 & 0x80u);
+        uint32_t cv = code_of(r[j], ev, (x >> 16 << 4) + 8u);
+        const uint32_t least = __float_as_uint(r[j]) < 1u ? __float_as_uint(r[j]) : 1u;        // a root above 0 keeps a code above 0
+        cv = cv < least ? least : cv;
+        if (any_odd) {
+            cm = finite(m[j]) ? cm : 0x7Fu;
+            cv = finite(r[j]) ? cv : 0x7Fu;
+        }
+        mc |= cm << (8 * j);
+        vc |= cv << (8 * j);
+    }
+    if constexpr (WHOLE) {
+        __builtin_memcpy(M, &mc, 4);
+        __builtin_memcpy(V, &vc, 4);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (j < left) {
+                M[j] = (uint8_t)(mc >> (8 * j));
+                V[j] = (uint8_t)(vc >> (8 * j));
+            }
+    }
+    if (lane == 0) {
+        *ms = (uint8_t)(em + 127);
+        *vs = (uint8_t)(ev + 127);
+    }
+}
+
+// a wave per block of 256; nothing is shared between waves
 template <typename T>
 __global__ __launch_bounds__(256) void adamw8_kernel(Table t, const Factors* __restrict__ factors, Rates k) {
-    constexpr int VEC = 4;                                    // elements per lane: a wave is one block of 256
     const int i = find_tensor(t.first, t.tensors, blockIdx.x);
     const long long n = t.n[i];
     const Factors f = factors[t.factors[i]];
     T* P = (T*)t.p[i];
     const T* G = (const T*)t.g[i];
     uint8_t *M = (uint8_t*)t.m[i], *V = (uint8_t*)t.v[i];
-    const int lane = threadIdx.x & 63;
-    long long s = (long long)(blockIdx.x - t.first[i]) * (AW_CHUNK / AW_STATE) + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    long long s = (long long)(blockIdx.x - t.first[i]) * (AW_CHUNK / AW_STATE) + wave;
     for (int it = 0; it < AW_CHUNK / AW_STATE / 4; ++it, s += 4) {
-        if (s * AW_STATE >= n) return;                        // whole waves; nothing is shared between waves
-        const long long c = s * AW_STATE + lane * VEC, left = n - c;
-        float p[VEC], g[VEC], m[VEC], r[VEC];
-        uint32_t mc = 0, vc = 0;
-        load_part<T, VEC>(P + c, left, p);
-        load_part<T, VEC>(G + c, left, g);
-        if (left >= VEC) {
-            __builtin_memcpy(&mc, M + c, 4);
-            __builtin_memcpy(&vc, V + c, 4);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (j < left) {
-                    mc |= (uint32_t)M[c + j] << (8 * j);
-                    vc |= (uint32_t)V[c + j] << (8 * j);
-                }
-        }
-        const float sm = pow2f((int)t.ms[i][s] - 127), sv = pow2f((int)t.vs[i][s] - 127);
-        m[0] = __builtin_amdgcn_cvt_f32_fp8(mc, 0) * sm;
-        m[1] = __builtin_amdgcn_cvt_f32_fp8(mc, 1) * sm;
-        m[2] = __builtin_amdgcn_cvt_f32_fp8(mc, 2) * sm;
-        m[3] = __builtin_amdgcn_cvt_f32_fp8(mc, 3) * sm;
-        r[0] = __builtin_amdgcn_cvt_f32_fp8(vc, 0) * sv;
-        r[1] = __builtin_amdgcn_cvt_f32_fp8(vc, 1) * sv;
-        r[2] = __builtin_amdgcn_cvt_f32_fp8(vc, 2) * sv;
-        r[3] = __builtin_amdgcn_cvt_f32_fp8(vc, 3) * sv;
-        float am = 0.f, ar = 0.f;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            float v = r[j] * r[j];
-            adamw_element(k, f, g[j], p[j], m[j], v, r[j]);
-            if (j < left) {
-                if (finite(m[j])) am = __builtin_fmaxf(am, __builtin_fabsf(m[j]));
-                if (finite(r[j])) ar = __builtin_fmaxf(ar, r[j]);
-            }
-        }
-        store_part<T, VEC>(P + c, left, p);
-        const int em = scale_exponent(wave_max(am)), ev = scale_exponent(wave_max(ar));
-        const float im = pow2f(-em), iv = pow2f(-ev);
-        mc = vc = 0;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const uint32_t x = random_bits(f.key, c + j);
-            mc |= code_of(m[j] * im, ((x & 0xFFFFu) << 4) + 8u, 0u) << (8 * j);
-            vc |= code_of(r[j] * iv, ((x >> 16) << 4) + 8u, r[j] > 0.f ? 1u : 0u) << (8 * j);
-        }
-        if (left >= VEC) {
-            __builtin_memcpy(M + c, &mc, 4);
-            __builtin_memcpy(V + c, &vc, 4);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (j < left) {
-                    M[c + j] = (uint8_t)(mc >> (8 * j));
-                    V[c + j] = (uint8_t)(vc >> (8 * j));
-                }
-        }
-        if (lane == 0) {
-            t.ms[i][s] = (uint8_t)(em + 127);
-            t.vs[i][s] = (uint8_t)(ev + 127);
-        }
+        const long long first = s * AW_STATE, c = first + lane * 4;
+        if (first >= n) return;
+        if (first + AW_STATE <= n) adamw8_block<T, true>(f, k, P + c, G + c, M + c, V + c, t.ms[i] + s, t.vs[i] + s, c, 0, lane);
+        else adamw8_block<T, false>(f, k, P + c, G + c, M + c, V + c, t.ms[i] + s, t.vs[i] + s, c, n - c, lane);
     }
 }
 
