@@ -188,6 +188,7 @@ class _LogProbsFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_logp, g_entropy, g_top, _):
+        ops.first_order_only("log_probs")
         logits, target, *rest = ctx.saved_tensors
         r = ops.LogProbs(*(rest.pop(0) if there else None for there in ctx.there))
         f32 = lambda g: None if g is None else g.float().contiguous()            # noqa: E731

@@ -1802,6 +1802,13 @@ def _elem(t, what):
     return code
 
 
+def first_order_only(what):
+    """called by a backward of a HIP operator: its result carries no history, so a second derivative would silently miss terms.  (The engine runs
+    a backward with gradients enabled exactly when it was asked for create_graph=True.)"""
+    if torch.is_grad_enabled():
+        raise W2CError("%s can be differentiated once only (create_graph=True)" % what)
+
+
 def _ln_affine(x, weight, bias, what):
     """(cols, element type of weight / bias) of a layer norm over x's last dimension"""
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -2102,7 +2109,8 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
         check(lib.w2c_adamw_step(rows.buffer_info()[0], n, bits, float(lr), _p(lr_dev), float(beta1), float(beta2), float(eps), float(weight_decay),
                                  _p(squares) if norm is not None else None, squares.numel() if norm is not None else 0, float(max_norm or 0.0),
                                  _p(norm), int(seed) & 0xFFFFFFFF, _p(ws), nbytes, _stream(dev)), "w2c_adamw_step")
-    torch.autograd.graph.increment_version(params)           # the engines' packed weights and autograd notice the in-place write
+    # the engines' packed weights and autograd notice the in-place write (inference tensors count no versions)
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
     return norm
 
 

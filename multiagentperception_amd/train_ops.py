@@ -349,6 +349,7 @@ class _LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dh):
+        ops.first_order_only("layer_norm")
         h, weight, bias, mean, rstd = ctx.saved_tensors
         dw = db = None
         if dy is None:                                   # only h was used
@@ -405,6 +406,7 @@ class _LinearFp8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        ops.first_order_only("linear_fp8")
         need_x, need_w, need_b = ctx.needs_input_grad
         rows = dy.reshape(-1, dy.shape[-1])
         q = ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous(), 1, rows=need_x, columns=need_w, sums=need_b)
