@@ -428,15 +428,16 @@ def linear_fp8(x, weight, bias=None):
     per 128 elements of the sum.  weight: [N, K] f32 / bf16 / f16, or ops.Fp8Blocks of it (quantize_fp8(weight, 128).rows: laid out once, for
     inference).  HIP kernels under the "hip" backend on GPU tensors, F.linear otherwise."""
     if isinstance(weight, ops.Fp8Blocks):
-        if x.requires_grad and torch.is_grad_enabled():
+        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise ops.W2CError("linear_fp8: quantised weights are for inference; pass the weights themselves to differentiate")
         if x.shape[-1] != weight.cols:
             raise ops.W2CError("linear_fp8: %d features against weights of %d" % (x.shape[-1], weight.cols))
         rows = x.reshape(-1, x.shape[-1])
-        y = ops.matmul_fp8(ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous()).rows, weight, bias, x.dtype)
+        y = ops.matmul_fp8(ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous()).rows, weight,
+                           None if bias is None else bias.detach().float().contiguous(), x.dtype)
         return y.view(x.shape[:-1] + (y.shape[1],))
     if _backend == "hip" and x.is_cuda:
-        if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or (bias is not None and tuple(bias.shape) != (weight.shape[0],)):
+        if weight.dim() != 2 or not weight.numel() or weight.shape[1] != x.shape[-1] or (bias is not None and tuple(bias.shape) != (weight.shape[0],)):
             raise ops.W2CError("linear_fp8: x %s, weight %s and bias do not fit" % (tuple(x.shape), tuple(weight.shape)))
         return _LinearFp8Fn.apply(x, weight, bias)
     return F.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))

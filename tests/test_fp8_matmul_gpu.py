@@ -190,6 +190,18 @@ def test_module_frozen_parts_and_no_rows():
     assert y.shape == (0, 24) and gx.shape == (0, 40) and not gw.any() and not gb.any()
 
 
+def test_quantised_weights_take_a_half_bias_and_a_frozen_module():
+    m = train_ops.LinearFp8(40, 24).cuda().bfloat16().requires_grad_(False)
+    x = torch.randn(6, 40, device="cuda", dtype=BF16)
+    held = ops.quantize_fp8(m.weight, 128).rows
+    assert torch.equal(train_ops.linear_fp8(x, held, m.bias), m(x))                 # the same operands in the same product
+    with pytest.raises(W2CError):
+        train_ops.linear_fp8(x, held, m.bias.clone().requires_grad_())
+    for w in (torch.zeros(0, 40, device="cuda"), torch.zeros(24, 0, device="cuda")):
+        with pytest.raises(W2CError):
+            train_ops.linear_fp8(x[:, :w.shape[1]], w)
+
+
 def test_replays_of_a_captured_linear_step():
     m = train_ops.LinearFp8(300, 200).cuda()
     x, dy = torch.randn(100, 300, device="cuda", requires_grad=True), torch.randn(100, 200, device="cuda")

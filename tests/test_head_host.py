@@ -57,6 +57,13 @@ def test_tensor_level_operators_refuse_the_cpu():
         opt.step()
 
 
+def test_quantised_weights_refuse_to_lose_a_gradient():
+    q = ops.Fp8Blocks(torch.zeros(4, 128, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros(4, 1, dtype=torch.uint8).view(torch.float8_e8m0fnu), 8)
+    for x, bias in ((torch.randn(3, 8), torch.zeros(4, requires_grad=True)), (torch.randn(3, 8, requires_grad=True), None)):
+        with pytest.raises(W2CError, match="inference"):
+            train_ops.linear_fp8(x, q, bias)
+
+
 P = 1 << 20                       # an address that a refused call never touches
 
 
