@@ -207,6 +207,8 @@ def log_probs(input, target=None, top=0, dim=-1, ignore_index=-100):
         rows = input.dim() == 2 and dim % 2 == 1 and input.stride(1) == 1 and input.stride(0) >= input.shape[1]
         return LogProbs(*_LogProbsFn.apply(input if rows else input.contiguous(), target, int(top), int(dim), int(ignore_index)))
     x = input.float().movedim(dim, -1)
+    if not 0 <= top <= min(x.shape[-1], ops.LOG_PROBS_TOP_MOST):
+        raise ops.W2CError("log_probs: top must lie in 0 .. min(classes, %d), got %d of %d classes" % (ops.LOG_PROBS_TOP_MOST, top, x.shape[-1]))
     empty = (x == -float("inf")).all(-1, keepdim=True)
     lp = torch.log_softmax(x.masked_fill(empty, 0.0), -1).masked_fill(empty, -float("inf"))
     p = lp.exp()

@@ -34,6 +34,12 @@ def test_log_probs_on_the_cpu():
     assert torch.equal(a.logp, b.logp) and torch.equal(a.top_index, b.top_index) and a.top_index.shape == (2, 3, 4, 2)
 
 
+@pytest.mark.parametrize("classes,top", [(4, 5), (40, 33), (4, -1)])
+def test_log_probs_on_the_cpu_refuses_what_the_kernels_refuse(classes, top):
+    with pytest.raises(W2CError, match="top must lie in"):
+        loss.log_probs(torch.randn(2, classes), top=top)
+
+
 def test_layers_on_the_cpu_are_the_stock_ones():
     torch.manual_seed(0)
     n, stock = train_ops.LayerNormHip(12), torch.nn.LayerNorm(12)
