@@ -1844,9 +1844,9 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None):
     return y, h, mean, rstd
 
 
-def layer_norm_backward(dy, h, weight, mean, rstd, dh=None, bias=True):
+def layer_norm_backward(dy, h, weight, mean, rstd, dh=None, bias=True, weight_grad=True):
     """-> (dx, dweight | None, dbias | None) of layer_norm_forward; dx is the gradient of x and of residual alike.  dh: the gradient that
-    reaches h by another way (the residual stream), added to dx.  weight None: no dweight (dbias then is f32)."""
+    reaches h by another way (the residual stream), added to dx.  weight None or weight_grad False: no dweight (without a weight dbias is f32)."""
     dev = _need_gpu(dy, h, weight, mean, rstd, dh)
     code = _elem(h, "layer_norm backward")
     cols, wtype = _ln_affine(h, weight, None, "layer_norm backward")
@@ -1857,7 +1857,7 @@ def layer_norm_backward(dy, h, weight, mean, rstd, dh=None, bias=True):
     if mean.numel() != rows or rstd.numel() != rows or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
         raise W2CError("layer_norm backward: mean and rstd must be f32, one per row")
     dx = torch.empty_like(h)
-    dw = torch.empty(cols, dtype=wtype, device=dev) if weight is not None else None
+    dw = torch.empty(cols, dtype=wtype, device=dev) if weight is not None and weight_grad else None
     db = torch.empty(cols, dtype=wtype, device=dev) if bias else None
     if not rows:
         for t in (dw, db):

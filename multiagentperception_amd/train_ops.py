@@ -357,7 +357,8 @@ class _LayerNormFn(torch.autograd.Function):
         else:
             want_b = bias is not None and ctx.needs_input_grad[2]
             dx, dw, db = ops.layer_norm_backward(dy.contiguous(), h, None if weight is None else weight.detach().contiguous(), mean, rstd,
-                                                 dh=None if dh is None else dh.contiguous(), bias=want_b)
+                                                 dh=None if dh is None else dh.contiguous(), bias=want_b,
+                                                 weight_grad=ctx.needs_input_grad[1])
             if want_b:
                 db = db.to(bias.dtype)
         return dx, dw, db, None, dx if ctx.has_res else None

@@ -150,6 +150,23 @@ def test_module_trains_like_the_formula_and_takes_strided_inputs():
     assert torch.equal(torch.autograd.grad(h.sum(), r)[0], torch.ones_like(r))               # only h is used
 
 
+def test_a_frozen_norm_hands_the_gradient_on():
+    m = train_ops.LayerNormHip(300).cuda()
+    x = torch.randn(40, 300, device="cuda", requires_grad=True)
+    dy = torch.randn(40, 300, device="cuda")
+    (want,) = torch.autograd.grad(m(x), x, dy)
+    got = []
+    for weight, bias in ((False, True), (True, False), (False, False)):
+        m.weight.requires_grad_(weight)
+        m.bias.requires_grad_(bias)
+        (gx, *rest) = torch.autograd.grad(m(x), [x] + [p for p in m.parameters() if p.requires_grad], dy)
+        assert torch.equal(gx, want)
+        got.append(rest)
+    m.requires_grad_(True)
+    dw, db = torch.autograd.grad(m(x), (m.weight, m.bias), dy)
+    assert torch.equal(got[0][0], db) and torch.equal(got[1][0], dw) and not got[2]
+
+
 def test_gradient_against_differences():
     g = torch.Generator().manual_seed(7)
     x, w, b, up = (torch.randn(s, generator=g).cuda() for s in ((3, 40), (40,), (40,), (3, 40)))
