@@ -520,7 +520,7 @@ int w2c_layer_norm_backward(const void* dy, const void* h, const void* dh, int d
                             w2c_stream_t stream);
 
 /* Log probability of a given class, entropy and the `top` largest alternatives of every row of logits, one read of them.
- * x: [outer, classes, inner]; inner = 1: rows of `row_stride` >= classes elements; inner > 1: dense (row_stride = classes * inner).  Rows are
+ * x: [outer, classes, inner]; inner = 1: rows of `row_stride` >= classes elements; inner > 1: dense (row_stride = classes * inner), at most 8 192 classes.  Rows are
  * numbered outer * inner.  target: int64 [rows] or NULL (then logp NULL); ignore_index there answers 0, any other value outside
  * [0, classes) NaN.  logp, entropy: f32 [rows]; top_logp f32, top_index int64 [rows, top], largest first, equal logits by the lower index
  * (top <= 32, <= classes; a NaN counts as -inf in this order); stats: f32 [rows, 2], for the backward.  -inf is a masked class; a row of nothing else

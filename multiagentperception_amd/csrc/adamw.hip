@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr int AW_TENSORS = 48;            // a launch's table: 48 x 60 bytes of the 4 KiB that kernel arguments may take
+constexpr int AW_TENSORS = 48;            // a launch's table: 48 x 64 bytes of the 4 KiB that kernel arguments may take
 constexpr int AW_STEPS = 256;             // step counters per launch
 constexpr int AW_STATE = 256;             // elements per 8-bit scale
 constexpr int AW_FIELDS = 9;              // of a tensor's row in the C ABI: p, g, m, v, m_scale, v_scale, step, n, dtype

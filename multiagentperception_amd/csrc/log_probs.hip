@@ -67,16 +67,15 @@ __device__ __forceinline__ Run wave_join(Run r) {
 
 // order of the alternatives: larger value first, then lower index; NaN ranks as -inf.  0 = none
 typedef unsigned long long key_t;
-__device__ __forceinline__ key_t key_of(float v, int index) {
+__device__ __forceinline__ uint32_t ordered(float v) {               // not below 2^22: -inf is 0x007FFFFF
     const uint32_t b = __float_as_uint(v == v ? v : -INFINITY);
     const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return ((key_t)(v == 0.f ? 0x80000000u : o) << 32) | (uint32_t)~index;          // -0 and +0 are one value
+    return v == 0.f ? 0x80000000u : o;                               // -0 and +0 are one value
 }
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
+__device__ __forceinline__ key_t key_of(float v, int index) { return (key_t)ordered(v) << 32 | (uint32_t)~index; }
 __device__ __forceinline__ int key_index(key_t k) { return (int)~(uint32_t)k; }
-__device__ __forceinline__ float key_value(key_t k) {
-    const uint32_t o = (uint32_t)(k >> 32);
-    return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
-}
+__device__ __forceinline__ float key_value(key_t k) { return unordered((uint32_t)(k >> 32)); }
 template <int CTRL, int ROWS>
 __device__ __forceinline__ key_t max_key_step(key_t k) {
     const key_t p = (key_t)dpp<CTRL, ROWS>(0u, (uint32_t)(k >> 32)) << 32 | dpp<CTRL, ROWS>(0u, (uint32_t)k);
@@ -117,6 +116,47 @@ __device__ __forceinline__ Stat row_answer(const Run& r, const Out& o, long long
 }
 
 // ---- lane per row ------------------------------------------------------------------------------------------------------------------------
+// The K largest of the classes a lane has walked, largest first; classes come in ascending order, so an equal one goes behind those before it.  A new
+// value x moves place k to the middle one of (place k - 1, x, place k): no chain from place to place.  bf16 and f16 values leave 13 bits of an
+// ordered f32 unused, and the class fits there (at most 8 192 of them): two instructions a place where f32 values take five.
+// 64 maps of 19 x 128 x 256, bf16 / f32, with 2, 5 and 16 alternatives: 51 / 53, 78 / 100 and 178 / 270 us (without any 36 / 41).
+constexpr int LP_LANE_CLASSES = 8192;
+template <typename T, int K>
+struct Largest {
+    static constexpr bool ONE = sizeof(T) == 2;
+    uint32_t v[K];
+    int at[ONE ? 1 : K];
+    __device__ __forceinline__ Largest() {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            v[k] = 0;
+            if constexpr (!ONE) at[k] = 0;
+        }
+    }
+    __device__ __forceinline__ void add(float value, int j, bool there) {
+        uint32_t x = ordered(value);
+        if constexpr (ONE) x = (x & ~(uint32_t)(LP_LANE_CLASSES - 1)) | (uint32_t)(LP_LANE_CLASSES - 1 - j);
+        x = there ? x : 0;
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k) {
+            if constexpr (!ONE) {
+                const int moved = k && x > v[k ? k - 1 : 0] ? at[k ? k - 1 : 0] : j;
+                at[k] = x > v[k] ? moved : at[k];
+            }
+            const uint32_t low = k && v[k ? k - 1 : 0] < x ? v[k ? k - 1 : 0] : x;
+            v[k] = low > v[k] ? low : v[k];
+        }
+    }
+    __device__ __forceinline__ int index(int k) const {
+        if constexpr (ONE) return LP_LANE_CLASSES - 1 - (int)(v[k] & (LP_LANE_CLASSES - 1));
+        else return at[k];
+    }
+    __device__ __forceinline__ float value(int k) const {
+        if constexpr (ONE) return unordered(v[k] & 0x80000000u ? v[k] & ~(uint32_t)(LP_LANE_CLASSES - 1) : v[k] | (LP_LANE_CLASSES - 1));
+        else return unordered(v[k]);
+    }
+};
+
 // row i of block row n: classes at x[n * outer_stride + i * row_stride + j * class_stride]
 template <typename T, int KMAX>
 __global__ __launch_bounds__(256) void lp_lane_forward_kernel(const T* __restrict__ x, long long P, long long outer, int C, long long outer_stride,
@@ -130,47 +170,57 @@ __global__ __launch_bounds__(256) void lp_lane_forward_kernel(const T* __restric
         const long long t = o.logp ? o.target[row] : -1;
         const float xt = t >= 0 && t < C ? to_f32(p[t * class_stride]) : 0.f;
         Run r{-INFINITY, 0.f, 0.f};
-        float tv[KMAX > 0 ? KMAX : 1];
-        int ti[KMAX > 0 ? KMAX : 1];
+        Largest<T, (KMAX > 0 ? KMAX : 1)> best;
+        T next[N];
+        auto fetch = [&](int j) {
 #pragma unroll
-        for (int k = 0; k < KMAX; ++k) {
-            tv[k] = -INFINITY;
-            ti[k] = -1;
-        }
+            for (int e = 0; e < N; ++e) next[e] = j + e < C ? p[(long long)(j + e) * class_stride] : from_f32<T>(-INFINITY);
+        };
+        fetch(0);
         for (int j = 0; j < C; j += N) {
             float v[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = j + e < C ? to_f32(p[(long long)(j + e) * class_stride]) : -INFINITY;
+            for (int e = 0; e < N; ++e) v[e] = to_f32(next[e]);
+            if (j + N < C) fetch(j + N);                       // on its way while this one is added up
             run_add<N>(r, v, max_of<N>(v));
             if constexpr (KMAX > 0) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    float cv = v[e] == v[e] ? v[e] : -INFINITY;
-                    int ci = j + e;
-                    if (ci < C && (cv > tv[KMAX - 1] || ti[KMAX - 1] < 0)) {
-                        bool in = false;                       // once in its place everything behind moves down, equal values too
-#pragma unroll
-                        for (int k = 0; k < KMAX; ++k) {
-                            in = in || cv > tv[k] || ti[k] < 0;
-                            const float sv = tv[k];
-                            const int si = ti[k];
-                            tv[k] = in ? cv : sv;
-                            ti[k] = in ? ci : si;
-                            cv = in ? sv : cv;
-                            ci = in ? si : ci;
-                        }
-                    }
-                }
+                for (int e = 0; e < N; ++e) best.add(v[e], j + e, j + e < C);
             }
         }
         const Stat s = row_answer(r, o, row, C, xt);
-        if constexpr (KMAX > 0) {
+        if constexpr (KMAX > 0 && KMAX <= 4) {
 #pragma unroll
             for (int k = 0; k < KMAX; ++k)
                 if (k < o.top) {
-                    o.top_logp[row * o.top + k] = (tv[k] - s.m) - s.logs;
-                    o.top_index[row * o.top + k] = ti[k];
+                    o.top_logp[row * o.top + k] = (best.value(k) - s.m) - s.logs;
+                    o.top_index[row * o.top + k] = best.index(k);
                 }
+        }
+        if constexpr (KMAX > 4) {
+            // the wave's rows' answers lie one behind the other: through LDS (rows an odd number of dwords apart) each store covers whole lines
+            // (64 x 19 x 128 x 256 bf16 with 8 alternatives 145 -> 87 us; up to 4 are stored as they are: 2 of them took 58 us this way, 51 directly)
+            extern __shared__ uint32_t staged[];
+            const int lane = threadIdx.x & 63, pitch = o.top | 1, there = P - (i - lane) < 64 ? (int)(P - (i - lane)) : 64;
+            uint32_t* mine = staged + (threadIdx.x >> 6) * 64 * pitch;
+            const uint32_t inverse = 0xFFFFFFFFu / (uint32_t)o.top + 1u;                   // q / top = umulhi(q, inverse) for q < 2^16
+            const long long first = (row - lane) * o.top;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int k = 0; k < KMAX; ++k)
+                    if (k < o.top) mine[lane * pitch + k] = half ? (uint32_t)best.index(k) : __float_as_uint((best.value(k) - s.m) - s.logs);
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                for (int q = lane; q < there * o.top; q += there) {
+                    const int of = (int)__umulhi((uint32_t)q, inverse);
+                    const uint32_t v = mine[of * pitch + q - of * o.top];
+                    if (half) o.top_index[first + q] = (int)v;
+                    else o.top_logp[first + q] = __uint_as_float(v);
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
         }
     }
 }
@@ -553,9 +603,11 @@ template <typename T>
 int lp_forward(const void* x, long long outer, int C, long long inner, long long row_stride, const Out& o, void* ws, hipStream_t st) {
     if (lp_lane(C, inner)) {
         const LaneGrid g = lane_grid(outer, C, inner, row_stride);
-#define LP_LANE(K) hipLaunchKernelGGL((lp_lane_forward_kernel<T, K>), g.grid, g.block, 0, st, (const T*)x, g.P, g.outer, C, g.outer_stride, g.row_stride, g.class_stride, o)
+        const size_t lds = o.top > 4 ? (size_t)g.block.x * (o.top | 1) * sizeof(uint32_t) : 0;
+#define LP_LANE(K) hipLaunchKernelGGL((lp_lane_forward_kernel<T, K>), g.grid, g.block, lds, st, (const T*)x, g.P, g.outer, C, g.outer_stride, g.row_stride, g.class_stride, o)
         if (o.top == 0) LP_LANE(0);
         else if (o.top <= 2) LP_LANE(2);
+        else if (o.top <= 4) LP_LANE(4);
         else if (o.top <= 8) LP_LANE(8);
         else LP_LANE(32);
 #undef LP_LANE
@@ -609,7 +661,7 @@ int lp_backward(const void* x, long long outer, int C, long long inner, long lon
 
 bool lp_shape_ok(int dtype, long long outer, int C, long long inner, long long row_stride) {
     return dtype >= W2C_F32 && dtype <= W2C_F16 && outer >= 1 && outer <= 0x7FFFFFFF && C >= 1 && C <= (1 << 28) && inner >= 1 &&
-           inner <= 0x7FFFFFFF && (inner > 1 ? row_stride == (long long)C * inner : row_stride >= C);
+           inner <= 0x7FFFFFFF && (inner == 1 || C <= LP_LANE_CLASSES) && (inner > 1 ? row_stride == (long long)C * inner : row_stride >= C);
 }
 
 }  // namespace

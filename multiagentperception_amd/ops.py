@@ -1996,8 +1996,8 @@ def _dense(t):
     return True
 
 
-_dtype, _device, _shape, _layout = (operator.attrgetter(n) for n in ("dtype", "device", "shape", "layout"))
-_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_dtype, _shape, _layout = (operator.attrgetter(n) for n in ("dtype", "shape", "layout"))
+_ptr, _numel, _contiguous, _index = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device      # (-1: on the CPU)
 
 
 def _rows(*columns):
@@ -2006,8 +2006,8 @@ def _rows(*columns):
 
 
 def _adamw_tensors(params, grads):
-    """(device, addresses of the gradients, elements, element types) after the checks of parameters and gradients.  (Attribute by attribute over
-    whole lists: a step of a small network is bound by these checks.)"""
+    """(device, addresses of the parameters and of the gradients, elements, element types) after the checks of parameters and gradients.
+    (Attribute by attribute over whole lists: a step of a small network is bound by these checks.)"""
     n = len(params)
     if not n or len(grads) != n:
         raise W2CError("adamw: as many gradients as parameters expected, at least one (got %d and %d)" % (len(grads), n))
@@ -2017,13 +2017,13 @@ def _adamw_tensors(params, grads):
     dtypes = list(map(_dtype, params))
     if not set(dtypes) <= _ELEM.keys() or dtypes != list(map(_dtype, grads)):
         raise W2CError("adamw: f32, bf16 or f16 parameters with gradients of their types expected")
-    if set(map(_layout, grads)) != {torch.strided} or list(map(_shape, params)) != list(map(_shape, grads)) or {dev} != {*map(_device, params), *map(_device, grads)}:
+    if set(map(_layout, grads)) != {torch.strided} or list(map(_shape, params)) != list(map(_shape, grads)) or {dev.index} != {*map(_index, params), *map(_index, grads)}:
         raise W2CError("adamw: dense gradients of the parameters' shapes on %s expected" % dev)
     if not (all(map(_contiguous, params)) and all(map(_contiguous, grads))):
         for i, (p, g) in enumerate(zip(params, grads)):
             if not (p.is_contiguous() and g.is_contiguous()) and (p.stride() != g.stride() or not _dense(p)):
                 raise W2CError("adamw: parameter %d and its gradient must be laid out alike, without gaps" % i)
-    return dev, list(map(_ptr, grads)), list(map(_numel, params)), [_ELEM[d] for d in dtypes]
+    return dev, list(map(_ptr, params)), list(map(_ptr, grads)), list(map(_numel, params)), list(map(_ELEM.__getitem__, dtypes))
 
 
 def _grad_squares(dev, rows, n):
@@ -2040,7 +2040,7 @@ def _grad_squares(dev, rows, n):
 
 def grad_squares(grads):
     """sums of the squares of parts of the gradients (f64), for adamw_step's `squares`: their total is the squared norm of all of them"""
-    dev, g, sizes, types = _adamw_tensors(grads, grads)
+    dev, _, g, sizes, types = _adamw_tensors(grads, grads)
     none = [0] * len(g)
     return _grad_squares(dev, _rows(none, g, none, none, none, none, none, sizes, types), len(g))
 
@@ -2053,22 +2053,22 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
                                 scales of ADAMW_STATE_BLOCK elements; rounded at random by (seed, step, place)
     lr: a number, or an f32 device tensor of one element (a captured step then follows it).  max_norm: the gradients are scaled down to this
     norm in all; `squares` (grad_squares) where more tensors than these share the norm.  -> the norm before that (f32 on the device), or None."""
-    dev, g, sizes, types = _adamw_tensors(params, grads)
+    dev, p, g, sizes, types = _adamw_tensors(params, grads)
     n = len(params)
     if len(states) != n or len(steps) != n or len({*map(len, states)}) != 1 or len(states[0]) not in (2, 4):
         raise W2CError("adamw: a step and a state, all (m, v) or all (m, m_scale, v, v_scale), for each of %d parameters expected" % n)
     bits = 32 if len(states[0]) == 2 else 8
     parts = list(zip(*states))
     for t in (*parts, steps):
-        if {*map(_device, t)} != {dev}:
+        if {*map(_index, t)} != {dev.index}:
             raise W2CError("adamw: the states and steps must be on %s" % dev)
     if bits == 32:
         for t in parts:
             if {*map(_dtype, t)} != {torch.float32} or list(map(_numel, t)) != sizes:
                 raise W2CError("adamw: f32 moments of the parameters' elements expected")
             if not (all(map(_contiguous, t)) and all(map(_contiguous, params))):
-                for i, (p, q) in enumerate(zip(params, t)):
-                    if not (p.is_contiguous() and q.is_contiguous()) and p.stride() != q.stride():
+                for i, (a, b) in enumerate(zip(params, t)):
+                    if not (a.is_contiguous() and b.is_contiguous()) and a.stride() != b.stride():
                         raise W2CError("adamw: parameter %d: its moments must be laid out like it" % i)
         m, v = (list(map(_ptr, t)) for t in parts)
         ms = vs = [0] * n
@@ -2084,7 +2084,7 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
     if {*map(_dtype, steps)} != {torch.float32} or {*map(_numel, steps)} != {1}:
         raise W2CError("adamw: steps must be one f32 element each")
     counters = list(map(_ptr, steps))
-    written = [a for a in (*map(_ptr, params), *held, *counters) if a]          # (a tensor without elements has no address)
+    written = [a for a in (*p, *held, *counters) if a]          # (a tensor without elements has no address)
     if len({*written}) != len(written):
         raise W2CError("adamw: a parameter, moment or step is in the lists twice")
     if max_norm is not None and not max_norm > 0:
@@ -2094,7 +2094,7 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
             raise W2CError("adamw: a tensor lr must be one f32 element on the parameters' device")
         lr_dev, lr = lr, 0.0
-    rows = _rows(map(_ptr, params), g, m, v, ms, vs, counters, sizes, types)
+    rows = _rows(p, g, m, v, ms, vs, counters, sizes, types)
     norm = None
     if max_norm is not None:
         if squares is None:
@@ -2109,8 +2109,8 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
         check(lib.w2c_adamw_step(rows.buffer_info()[0], n, bits, float(lr), _p(lr_dev), float(beta1), float(beta2), float(eps), float(weight_decay),
                                  _p(squares) if norm is not None else None, squares.numel() if norm is not None else 0, float(max_norm or 0.0),
                                  _p(norm), int(seed) & 0xFFFFFFFF, _p(ws), nbytes, _stream(dev)), "w2c_adamw_step")
-    # the engines' packed weights and autograd notice the in-place write (inference tensors count no versions)
-    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+    # the engines' packed weights and autograd notice the in-place write
+    torch.autograd.graph.increment_version(params)
     return norm
 
 

@@ -91,7 +91,7 @@ def test_layer_norm_backward_refuses(lib, change):
 
 @pytest.mark.parametrize("change", [dict(x=0), dict(entropy=0), dict(stats=0), dict(dtype=3), dict(outer=0), dict(outer=1 << 31), dict(C=0), dict(C=(1 << 28) + 1), dict(inner=0),
                                     dict(stride=9999), dict(target=0), dict(logp=0), dict(top=-1), dict(top=33), dict(C=4, stride=4, top=5), dict(tl=0), dict(ti=0),
-                                    dict(ws=0), dict(nbytes=3), dict(ws=P + 4), dict(inner=2, stride=10000)])
+                                    dict(ws=0), dict(nbytes=3), dict(ws=P + 4), dict(inner=2, stride=10000), dict(inner=2, C=8193, stride=16386)])
 def test_log_probs_forward_refuses(lib, change):
     a = dict(x=P, dtype=1, outer=3, C=10000, inner=1, stride=10000, target=P, top=4, logp=P, entropy=P, tl=P, ti=P, stats=P, ws=P,
              nbytes=lib.w2c_log_probs_workspace_bytes(3, 10000, 1, 4))
