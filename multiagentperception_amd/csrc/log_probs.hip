@@ -441,7 +441,13 @@ struct RowGrad {
     float m, logs, a, c0, c1;
     int t;                                    // -1: none
 };
-__device__ __forceinline__ RowGrad row_grad(const Grad& g, long long row, int C) {
+__device__ __forceinline__ float top_grads(const Grad& g, long long row) {
+    float sum = 0.f;
+    if (g.g_top)
+        for (int i = 0; i < g.top; ++i) sum += g.g_top[row * g.top + i];
+    return sum;
+}
+__device__ __forceinline__ RowGrad row_grad(const Grad& g, long long row, int C, float sum_of_top) {
     RowGrad r;
     r.m = g.stats[2 * row];
     r.logs = g.stats[2 * row + 1];
@@ -455,9 +461,7 @@ __device__ __forceinline__ RowGrad row_grad(const Grad& g, long long row, int C)
             r.t = in ? (int)t : -1;
         }
     }
-    float whole = r.a;
-    if (g.g_top)
-        for (int i = 0; i < g.top; ++i) whole += g.g_top[row * g.top + i];
+    const float whole = r.a + sum_of_top;
     const float c = g.g_entropy ? g.g_entropy[row] : 0.f;
     r.c1 = -c;
     r.c0 = -fmaf(c, g.entropy[row], whole);
@@ -470,19 +474,22 @@ __device__ __forceinline__ float class_grad(const RowGrad& r, float x) {
 }
 // the places that get more than that: lane 0 the target's, lane 1 + i the i-th alternative's (the same place: the same value)
 template <typename T>
-__device__ __forceinline__ void place_grad(const RowGrad& r, const Grad& g, long long row, int C, int lane, long long lo, long long hi, const T* p,
-                                           T* d, long long class_stride) {
+__device__ __forceinline__ void place_grad(const RowGrad& r, const Grad& g, long long row, int lane, long long lo, long long hi, const T* p,
+                                           T* d) {
     const int top = g.g_top ? g.top : 0;
     if (lane > top || r.logs == INFINITY) return;
     const long long j = lane ? g.top_index[row * top + lane - 1] : r.t;
     if (j < lo || j >= hi) return;
-    float v = class_grad(r, to_f32(p[j * class_stride])) + (j == r.t ? r.a : 0.f);
+    float v = class_grad(r, to_f32(p[j])) + (j == r.t ? r.a : 0.f);
     for (int i = 0; i < top; ++i)
         if (g.top_index[row * top + i] == j) v += g.g_top[row * top + i];
-    d[j * class_stride] = from_f32<T>(v);
+    d[j] = from_f32<T>(v);
 }
 
-// KMAX alternatives in registers, their places compared with every class; KMAX = 0 with alternatives: those places are written again
+__device__ __forceinline__ uint32_t class_or_none(long long j, int C) { return j >= 0 && j < C ? (uint32_t)j : 0xFFFFFFFFu; }
+// KMAX alternatives in registers, their places compared with every class.  More than 4 come through LDS, so that whole lines are read (as in the
+// forward kernel).  The next classes are on their way while these are stored: a store could alias them, so the compiler would not do it.
+// (64 maps of 19 x 128 x 256, bf16 / f32: 40 / 69 us without alternatives, 51 / 79 with 2, 111 / 116 with 5, 300 / 308 with 16)
 template <typename T, int KMAX>
 __global__ __launch_bounds__(256) void lp_lane_backward_kernel(const T* __restrict__ x, long long P, long long outer, int C, long long outer_stride,
                                                                long long row_stride, long long class_stride, Grad g, T* __restrict__ dx,
@@ -494,34 +501,66 @@ __global__ __launch_bounds__(256) void lp_lane_backward_kernel(const T* __restri
         const long long row = n * P + i;
         const T* p = x + n * outer_stride + i * row_stride;
         T* d = dx + n * dx_outer_stride + i * dx_row_stride;
-        const RowGrad r = row_grad(g, row, C);
-        float b[KMAX > 0 ? KMAX : 1];
-        int at[KMAX > 0 ? KMAX : 1];
+        T next[N];
+        auto fetch = [&](int j) {
 #pragma unroll
-        for (int k = 0; k < KMAX; ++k) {
-            const bool there = k < g.top && r.logs != INFINITY;
-            at[k] = there ? (int)g.top_index[row * g.top + k] : -1;
-            b[k] = there ? g.g_top[row * g.top + k] : 0.f;
+            for (int e = 0; e < N; ++e)
+                if (j + e < C) next[e] = p[(long long)(j + e) * class_stride];
+        };
+        fetch(0);
+        float b[KMAX > 0 ? KMAX : 1], sum = 0.f;
+        int at[KMAX > 0 ? KMAX : 1];
+        if constexpr (KMAX > 4) {
+            extern __shared__ uint32_t staged[];
+            const int lane = threadIdx.x & 63, pitch = g.top | 1, there = P - (i - lane) < 64 ? (int)(P - (i - lane)) : 64;
+            uint32_t* mine = staged + (threadIdx.x >> 6) * 64 * pitch;
+            const uint32_t inverse = 0xFFFFFFFFu / (uint32_t)g.top + 1u;
+            const long long first = (row - lane) * g.top;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                for (int q = lane; q < there * g.top; q += there) {
+                    const int of = (int)__umulhi((uint32_t)q, inverse);
+                    mine[of * pitch + q - of * g.top] = half ? class_or_none(g.top_index[first + q], C) : __float_as_uint(g.g_top[first + q]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+                for (int k = 0; k < KMAX; ++k) {
+                    const uint32_t v = k < g.top ? mine[lane * pitch + k] : 0u;
+                    if (half) at[k] = k < g.top ? (int)v : -1;
+                    else b[k] = __uint_as_float(v);
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KMAX; ++k) {
+                at[k] = k < g.top ? (int)class_or_none(g.top_index[row * g.top + k], C) : -1;
+                b[k] = k < g.top ? g.g_top[row * g.top + k] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KMAX; ++k) sum += b[k];
+        const RowGrad r = row_grad(g, row, C, sum);
+        if (r.logs == INFINITY) {                              // a row of masked classes has no gradient
+#pragma unroll
+            for (int k = 0; k < KMAX; ++k) b[k] = 0.f;
         }
         for (int j = 0; j < C; j += N) {
             float v[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (j + e < C) v[e] = to_f32(p[(long long)(j + e) * class_stride]);
+            for (int e = 0; e < N; ++e) v[e] = to_f32(next[e]);
+            if (j + N < C) fetch(j + N);
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 if (j + e < C) {
-                    float w = class_grad(r, v[e]);
-                    if constexpr (KMAX > 0) {
-                        w += j + e == r.t ? r.a : 0.f;
+                    float w = class_grad(r, v[e]) + (j + e == r.t ? r.a : 0.f);
 #pragma unroll
-                        for (int k = 0; k < KMAX; ++k) w += j + e == at[k] ? b[k] : 0.f;
-                    } else if (!g.g_top) w += j + e == r.t ? r.a : 0.f;
+                    for (int k = 0; k < KMAX; ++k) w += j + e == at[k] ? b[k] : 0.f;
                     d[(long long)(j + e) * class_stride] = from_f32<T>(w);
                 }
         }
-        if (KMAX == 0 && g.g_top)
-            for (int k = 0; k <= g.top; ++k) place_grad<T>(r, g, row, C, k, 0, C, p, d, class_stride);
     }
 }
 
@@ -536,7 +575,7 @@ __global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restric
     const T* p = x + row * row_stride;
     T* d = dx + row * C;
     const int lo = blockIdx.y * part_len, hi = C - lo < part_len ? C : lo + part_len;
-    const RowGrad r = row_grad(g, row, C);
+    const RowGrad r = row_grad(g, row, C, top_grads(g, row));
     auto take = [&](float (&v)[VEC]) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = class_grad(r, v[e]);
@@ -568,7 +607,7 @@ __global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restric
     // (behind the block's stores to these places)
     if constexpr (NW > 1) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-    place_grad<T>(r, g, row, C, t, lo, hi, p, d, 1);
+    place_grad<T>(r, g, row, t, lo, hi, p, d);
 }
 
 // few long rows: enough parts for about four blocks on every CU, none under 256 lanes' accesses of 16 bytes
@@ -635,12 +674,16 @@ template <typename T>
 int lp_backward(const void* x, long long outer, int C, long long inner, long long row_stride, const Grad& g, void* dx, hipStream_t st) {
     if (lp_lane(C, inner)) {
         const LaneGrid l = lane_grid(outer, C, inner, row_stride);
+        const int top = g.g_top ? g.top : 0;
+        const size_t lds = top > 4 ? (size_t)l.block.x * (top | 1) * sizeof(uint32_t) : 0;
 #define LP_LANE(K)                                                                                                                                \
-    hipLaunchKernelGGL((lp_lane_backward_kernel<T, K>), l.grid, l.block, 0, st, (const T*)x, l.P, l.outer, C, l.outer_stride, l.row_stride,          \
+    hipLaunchKernelGGL((lp_lane_backward_kernel<T, K>), l.grid, l.block, lds, st, (const T*)x, l.P, l.outer, C, l.outer_stride, l.row_stride,          \
                        l.class_stride, g, (T*)dx, l.outer_stride, inner > 1 ? 1ll : (long long)C)
-        if (!g.g_top || g.top > 8) LP_LANE(0);
-        else if (g.top <= 2) LP_LANE(2);
-        else LP_LANE(8);
+        if (top == 0) LP_LANE(0);
+        else if (top <= 2) LP_LANE(2);
+        else if (top <= 4) LP_LANE(4);
+        else if (top <= 8) LP_LANE(8);
+        else LP_LANE(32);
 #undef LP_LANE
         return w2c_launch_status();
     }
