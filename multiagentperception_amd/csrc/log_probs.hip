@@ -13,7 +13,7 @@
 //   wave per row   up to 2 048 contiguous classes
 //   block per row or per part of a row   longer; few long rows are split over blocks and joined by a second launch
 // Alternatives of the last two: every thread keeps the largest (value, index) of what it read; the k-th largest of those is a bound that
-// at most k threads reach, and only they look through their values again.
+// at most k threads reach, and only their values are looked through again.
 #include "lm_common.h"
 
 namespace {
@@ -76,19 +76,19 @@ __device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(
 __device__ __forceinline__ key_t key_of(float v, int index) { return (key_t)ordered(v) << 32 | (uint32_t)~index; }
 __device__ __forceinline__ int key_index(key_t k) { return (int)~(uint32_t)k; }
 __device__ __forceinline__ float key_value(key_t k) { return unordered((uint32_t)(k >> 32)); }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ key_t max_key_step(key_t k) {
-    const key_t p = (key_t)dpp<CTRL, ROWS>(0u, (uint32_t)(k >> 32)) << 32 | dpp<CTRL, ROWS>(0u, (uint32_t)k);
-    return p > k ? p : k;
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+    return wave_reduce(v, [](uint32_t a, auto ctrl, auto rows) {
+        const uint32_t p = dpp<decltype(ctrl)::value, decltype(rows)::value>(0u, a);
+        return p > a ? p : a;
+    });
 }
+// of all 64 lanes: the largest value, then the lowest index of the lanes that have it (mostly one)
 __device__ __forceinline__ key_t wave_max_key(key_t k) {
-    k = max_key_step<0x111, 0xF>(k);
-    k = max_key_step<0x112, 0xF>(k);
-    k = max_key_step<0x114, 0xF>(k);
-    k = max_key_step<0x118, 0xF>(k);
-    k = max_key_step<0x142, 0xA>(k);
-    k = max_key_step<0x143, 0xC>(k);
-    return (key_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, 63);
+    const uint32_t value = (uint32_t)(k >> 32), best = wave_max_bits(value);
+    const unsigned long long have = __ballot(value == best);
+    const uint32_t index = have & (have - 1) ? wave_max_bits(value == best ? (uint32_t)k : 0u)
+                                             : (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, __builtin_ctzll(have));
+    return (key_t)best << 32 | index;
 }
 
 struct Out {                                  // where a row's answers go
@@ -226,12 +226,32 @@ __global__ __launch_bounds__(256) void lp_lane_forward_kernel(const T* __restric
 }
 
 // ---- wave or block per (part of a) row -----------------------------------------------------------------------------------------------------
-// The top keys of NW waves' rows' parts, by rounds of the largest: `mine` is a lane's key; afterwards lane l < k of the FIRST wave holds the
-// l-th largest of the block's elements >= the bound.  lists: k * k keys, firsts: NW * k keys, both in shared memory.
+// what top_keys keeps in shared memory for a row: candidates or lists | (NW > 1: every wave's k first keys) | the threads that look again | counts
+constexpr int LP_CANDIDATES = 128;
+template <int NW> __host__ __device__ constexpr int top_keys_words(int k) {
+    return (k * k > LP_CANDIDATES ? k * k : LP_CANDIDATES) + (NW > 1 ? NW * k : 0) + k / 2 + 2;
+}
+template <int NW>
+__device__ __forceinline__ void row_barrier() {
+    if constexpr (NW > 1) __syncthreads();
+    else {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+// Lane l < k of the FIRST wave gets the l-th largest of the part's elements; `mine`: the largest key of what this thread read, with the first place
+// of its access in place of its own.  The k-th largest of those is a bound (accesses do not overlap, so these keys come in the order of places, and each of
+// the k largest threads has an element in front of any element of the others); the elements of these k threads from the bound on are
+// gathered by all threads, and their k largest taken by rounds.  Should more than 128 qualify (ascending rows), each of the k threads makes a
+// list of its own k largest instead.
 template <typename T, int NW>
-__device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int hi, int first, key_t mine, int k, key_t* lists, key_t* firsts, int* count) {
+__device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int hi, int origin, key_t mine, int k, key_t* lists) {
     constexpr int VEC = ElemOf<T>::VEC, TPR = NW * 64;
-    const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : threadIdx.x >> 6, t = NW == 1 ? lane : threadIdx.x;
+    key_t* firsts = lists + (k * k > LP_CANDIDATES ? k * k : LP_CANDIDATES);
+    int* chosen = (int*)(firsts + (NW > 1 ? NW * k : 0));
+    int* counts = chosen + (k / 2) * 2 + 2;              // [0] threads, [1] elements
     key_t left = mine, bound = 0;
     for (int r = 0; r < k; ++r) {                        // this wave's k largest thread keys
         bound = wave_max_key(left);
@@ -239,28 +259,71 @@ __device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int h
         if constexpr (NW > 1)
             if (lane == 0) firsts[wave * k + r] = bound;
     }
-    if constexpr (NW > 1) {
-        if (threadIdx.x == 0) *count = 0;
-        __syncthreads();
-        if (wave == 0) {                                 // the k-th largest of all waves' firsts
-            int at = 0;                                  // lane w < NW walks wave w's sorted list
-            for (int r = 0; r < k; ++r) {
-                const key_t head = lane < NW && at < k ? firsts[lane * k + at] : 0;
-                bound = wave_max_key(head);
-                if (head == bound) ++at;
-            }
-            if (lane == 0) firsts[0] = bound;            // (read by this wave only, above, before this write)
+    if (t == 0) counts[0] = counts[1] = 0;
+    row_barrier<NW>();
+    if constexpr (NW > 1) {                              // every wave finds the k-th largest of all of them
+        static_assert(NW == 4 && LP_TOP_MOST <= 32, "two keys a lane");
+        key_t a = lane < NW * k ? firsts[lane] : 0, b = lane + 64 < NW * k ? firsts[lane + 64] : 0;
+        if (a < b) {
+            const key_t c = a;
+            a = b;
+            b = c;
         }
-        __syncthreads();
-        bound = firsts[0];
-    } else {
-        if (lane == 0) *count = 0;
-        __builtin_amdgcn_wave_barrier();
+        for (int r = 0; r < k; ++r) {
+            bound = wave_max_key(a);
+            if (a == bound) {
+                a = b;
+                b = 0;
+            }
+        }
     }
-    if (mine && mine >= bound) {                         // at most k threads
-        key_t* list = lists + (long long)atomicAdd(count, 1) * k;
+    const bool again = mine && mine >= bound;            // at most k threads
+    if (again) chosen[atomicAdd(&counts[0], 1)] = t;
+    bound -= bound ? VEC - 1 : 0;                        // elements count from the end of the bound's access
+    row_barrier<NW>();
+    const int threads = counts[0], each = (hi - origin + TPR * VEC - 1) / (TPR * VEC);
+    for (int w = t; w < threads * each; w += TPR) {
+        const int turn = w / threads, c = origin + (turn * TPR + chosen[w - turn * threads]) * VEC;
+        float v[VEC];
+        load_range<T, VEC>(p, c, lo, hi, v, 0.f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const key_t q = c + e >= lo && c + e < hi ? key_of(v[e], c + e) : 0;
+            if (q && q >= bound) {
+                const int at = atomicAdd(&counts[1], 1);
+                if (at < LP_CANDIDATES) lists[at] = q;
+            }
+        }
+    }
+    row_barrier<NW>();
+    key_t answer = 0;
+    const int found = counts[1];
+    if (found <= LP_CANDIDATES) {
+        if (wave == 0) {
+            key_t a = lane < found ? lists[lane] : 0, b = lane + 64 < found ? lists[lane + 64] : 0;
+            if (a < b) {
+                const key_t c = a;
+                a = b;
+                b = c;
+            }
+            for (int r = 0; r < k; ++r) {
+                const key_t best = wave_max_key(a);
+                if (lane == r) answer = best;
+                if (a == best) {
+                    a = b;
+                    b = 0;
+                }
+            }
+        }
+        return answer;
+    }
+    row_barrier<NW>();                                   // (the lists overlay the candidates)
+    if (again) {
+        int which = 0;
+        while (chosen[which] != t) ++which;
+        key_t* list = lists + which * k;
         int n = 0;
-        for (int c = first; c < hi; c += TPR * VEC) {
+        for (int c = origin + t * VEC; c < hi; c += TPR * VEC) {
             float v[VEC];
             load_range<T, VEC>(p, c, lo, hi, v, 0.f);
 #pragma unroll
@@ -275,18 +338,11 @@ __device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int h
         }
         for (; n < k; ++n) list[n] = 0;
     }
-    if constexpr (NW > 1) __syncthreads();
-    else {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-    }
-    key_t answer = 0;
+    row_barrier<NW>();
     if (wave == 0) {
-        const int lists_n = *count;
         int at = 0;
         for (int r = 0; r < k; ++r) {
-            const key_t head = lane < lists_n && at < k ? lists[lane * k + at] : 0;
+            const key_t head = lane < threads && at < k ? lists[lane * k + at] : 0;
             const key_t best = wave_max_key(head);
             if (head == best && head) ++at;
             if (lane == r) answer = best;
@@ -301,7 +357,7 @@ template <typename T, int NW>
 __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int part_len,
                                                              Out o, float* __restrict__ parts, key_t* __restrict__ part_keys) {
     constexpr int VEC = ElemOf<T>::VEC, TPR = NW * 64, ROWS = 256 / TPR;
-    extern __shared__ key_t shared[];                    // per row: k * k lists | (NW > 1: NW * k firsts) | count
+    extern __shared__ key_t shared[];                    // top_keys_words per row
     __shared__ float slots[3][NW];
     const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6, k = o.top;
     const long long row = (long long)blockIdx.x * ROWS + (NW == 1 ? wave : 0);
@@ -311,14 +367,12 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
     Run r{-INFINITY, 0.f, 0.f};
     const int first = lo - misaligned(p + lo) + t * VEC;
     float best = -INFINITY;
-    int at = first < lo ? lo : first;
+    int at = first;                                      // the access that brought it first
     auto take = [&](const float (&v)[VEC], int c) {
         const float cm = max_of<VEC>(v);
-        if (k && cm > best) {
-            best = cm;
-#pragma unroll
-            for (int e = VEC - 1; e >= 0; --e)
-                if (v[e] == cm) at = c + e;
+        if (k) {
+            at = cm > best ? c : at;
+            best = __builtin_fmaxf(cm, best);
         }
         run_add<VEC>(r, v, cm);
     };
@@ -377,9 +431,9 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
         }
     }
     if (!k) return;
-    key_t* mem = shared + (NW == 1 ? wave * (k * k + 1) : 0);
-    const key_t mine = first < hi ? key_of(best, at) : 0;
-    const key_t q = top_keys<T, NW>(p, lo, hi, first, mine, k, mem, mem + k * k, (int*)(mem + k * k + (NW == 1 ? 0 : NW * k)));
+    key_t* mem = shared + (NW == 1 ? wave * top_keys_words<NW>(k) : 0);
+    const key_t mine = first < hi ? key_of(best, at < lo ? lo : at) : 0;
+    const key_t q = top_keys<T, NW>(p, lo, hi, lo - misaligned(p + lo), mine, k, mem);
     if (wave == 0 || NW == 1) {
         s.m = __shfl(s.m, 0, 64);
         s.logs = __shfl(s.logs, 0, 64);
@@ -654,7 +708,7 @@ int lp_forward(const void* x, long long outer, int C, long long inner, long long
     }
     const int k = o.top;
     if (C <= LP_WAVE_MOST) {
-        hipLaunchKernelGGL((lp_row_forward_kernel<T, 1>), dim3((unsigned)((outer + 3) / 4)), dim3(256), (size_t)4 * (k * k + 1) * sizeof(key_t), st,
+        hipLaunchKernelGGL((lp_row_forward_kernel<T, 1>), dim3((unsigned)((outer + 3) / 4)), dim3(256), (size_t)(k ? 4 * top_keys_words<1>(k) * sizeof(key_t) : 0), st,
                            (const T*)x, outer, C, row_stride, C, o, (float*)nullptr, (key_t*)nullptr);
         return w2c_launch_status();
     }
@@ -662,7 +716,7 @@ int lp_forward(const void* x, long long outer, int C, long long inner, long long
     const int len = n > 1 ? lp_part_len(C, n) : C, used = (int)(((long long)C + len - 1) / len);
     key_t* keys = n > 1 ? (key_t*)ws : nullptr;
     float* parts = n > 1 ? (float*)(keys + (long long)outer * n * k) : nullptr;
-    hipLaunchKernelGGL((lp_row_forward_kernel<T, 4>), dim3((unsigned)outer, used), dim3(256), (size_t)(k * k + 4 * k + 1) * sizeof(key_t), st,
+    hipLaunchKernelGGL((lp_row_forward_kernel<T, 4>), dim3((unsigned)outer, used), dim3(256), (size_t)(k ? top_keys_words<4>(k) * sizeof(key_t) : 0), st,
                        (const T*)x, outer, C, row_stride, len, o, parts, keys);
     if (n > 1)
         hipLaunchKernelGGL((lp_join_kernel<T>), dim3((unsigned)((outer + 3) / 4)), dim3(256), 0, st, (const T*)x, outer, C, row_stride, used, o,

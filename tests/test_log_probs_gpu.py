@@ -125,6 +125,21 @@ def test_ascending_and_descending_rows(C):
         assert torch.equal(r.top_index, v.sort(dim=1, descending=True, stable=True)[1][:, :20]) and r.logp is None
 
 
+@pytest.mark.parametrize("top", [1, 31, 32])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("C", [257, 1999, 9001, 40000])
+def test_rows_with_many_equal_or_rising_values(C, dtype, top):
+    """hundreds of values reach the bound that the alternatives are looked for from"""
+    i = torch.arange(C, device="cuda")
+    access, threads = i // (4 if dtype == F32 else 8), 64 if C <= 2048 else 256
+    column = access % threads
+    rows = torch.stack([torch.ones(C, device="cuda"), (i // 3).float(), (column < 31) * 10.0 + (column == 31) * 5.0, torch.where(i % 5 == 0, -INF, 1.0)]).to(dtype)
+    wide = torch.zeros(4, C + 3, dtype=dtype, device="cuda")
+    wide[:, :C] = rows
+    for x in (rows, wide[:, :C]):
+        assert torch.equal(ops.log_probs_forward(x, None, top).top_index, rows.float().sort(dim=1, descending=True, stable=True)[1][:, :top])
+
+
 def test_large_logits_keep_their_digits():
     _check(4, 500, 1, F32, 3, seed=1, spread=2000.0)
     _check(3, 20000, 1, F32, 3, seed=2, spread=2000.0)
