@@ -102,16 +102,14 @@ struct Out {                                  // where a row's answers go
 struct Stat {
     float m, logs;
 };
-__device__ __forceinline__ Stat row_answer(const Run& r, const Out& o, long long row, int C, float xt) {
+// t, xt: the row's target and its logit
+__device__ __forceinline__ Stat row_answer(const Run& r, const Out& o, long long row, int C, long long t, float xt) {
     const bool empty = r.m == -INFINITY && r.s == 0.f;
     const float m = r.m == -INFINITY ? 0.f : r.m, logs = empty ? INFINITY : logf(r.s);
     o.stats[2 * row] = m;
     o.stats[2 * row + 1] = logs;
     o.entropy[row] = empty ? 0.f : logs - r.u / r.s;
-    if (o.logp) {
-        const long long t = o.target[row];
-        o.logp[row] = t == o.ignore ? 0.f : t < 0 || t >= C ? __builtin_nanf("") : (xt - m) - logs;
-    }
+    if (o.logp) o.logp[row] = t == o.ignore ? 0.f : t < 0 || t >= C ? __builtin_nanf("") : (xt - m) - logs;
     return Stat{m, logs};
 }
 
@@ -188,7 +186,7 @@ __global__ __launch_bounds__(256) void lp_lane_forward_kernel(const T* __restric
                 for (int e = 0; e < N; ++e) best.add(v[e], j + e, j + e < C);
             }
         }
-        const Stat s = row_answer(r, o, row, C, xt);
+        const Stat s = row_answer(r, o, row, C, t, xt);
         if constexpr (KMAX > 0 && KMAX <= 4) {
 #pragma unroll
             for (int k = 0; k < KMAX; ++k)
@@ -364,6 +362,8 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
     if (row >= rows) return;                             // whole waves, and only where no barrier follows
     const T* p = x + row * row_stride;
     const int lo = blockIdx.y * part_len, hi = C - lo < part_len ? C : lo + part_len;
+    const long long target = o.logp && !parts ? o.target[row] : -1;     // (here, not behind the sums: two trips to memory, one behind the other)
+    const float xt = target >= 0 && target < C ? to_f32(p[target]) : 0.f;
     Run r{-INFINITY, 0.f, 0.f};
     const int first = lo - misaligned(p + lo) + t * VEC;
     float best = -INFINITY;
@@ -425,10 +425,7 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
             q[0] = r.m;
             q[1] = r.s;
             q[2] = r.u;
-        } else {
-            const long long g = o.logp ? o.target[row] : -1;
-            s = row_answer(r, o, row, C, g >= 0 && g < C ? to_f32(p[g]) : 0.f);
-        }
+        } else s = row_answer(r, o, row, C, target, xt);
     }
     if (!k) return;
     key_t* mem = shared + (NW == 1 ? wave * top_keys_words<NW>(k) : 0);
@@ -454,6 +451,8 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const T* __restrict__ x, l
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, k = o.top;
     if (row >= rows) return;
+    const long long target = o.logp ? o.target[row] : -1;
+    const float xt = target >= 0 && target < C ? to_f32(x[row * row_stride + target]) : 0.f;
     Run r{-INFINITY, 0.f, 0.f};
     if (lane < n_parts) {
         const float* q = parts + (row * n_parts + lane) * 3;
@@ -461,10 +460,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const T* __restrict__ x, l
     }
     r = wave_join(r);
     Stat s{0.f, 0.f};
-    if (lane == 0) {
-        const long long g = o.logp ? o.target[row] : -1;
-        s = row_answer(r, o, row, C, g >= 0 && g < C ? to_f32(x[row * row_stride + g]) : 0.f);
-    }
+    if (lane == 0) s = row_answer(r, o, row, C, target, xt);
     if (!k) return;
     s.m = __shfl(s.m, 0, 64);
     s.logs = __shfl(s.logs, 0, 64);
@@ -495,12 +491,6 @@ struct RowGrad {
     float m, logs, a, c0, c1;
     int t;                                    // -1: none
 };
-__device__ __forceinline__ float top_grads(const Grad& g, long long row) {
-    float sum = 0.f;
-    if (g.g_top)
-        for (int i = 0; i < g.top; ++i) sum += g.g_top[row * g.top + i];
-    return sum;
-}
 __device__ __forceinline__ RowGrad row_grad(const Grad& g, long long row, int C, float sum_of_top) {
     RowGrad r;
     r.m = g.stats[2 * row];
@@ -526,20 +516,6 @@ __device__ __forceinline__ float class_grad(const RowGrad& r, float x) {
     const float l = (x - r.m) - r.logs;
     return exp_d(l) * fmaf(r.c1, __builtin_fmaxf(l, LP_FLOOR), r.c0);
 }
-// the places that get more than that: lane 0 the target's, lane 1 + i the i-th alternative's (the same place: the same value)
-template <typename T>
-__device__ __forceinline__ void place_grad(const RowGrad& r, const Grad& g, long long row, int lane, long long lo, long long hi, const T* p,
-                                           T* d) {
-    const int top = g.g_top ? g.top : 0;
-    if (lane > top || r.logs == INFINITY) return;
-    const long long j = lane ? g.top_index[row * top + lane - 1] : r.t;
-    if (j < lo || j >= hi) return;
-    float v = class_grad(r, to_f32(p[j])) + (j == r.t ? r.a : 0.f);
-    for (int i = 0; i < top; ++i)
-        if (g.top_index[row * top + i] == j) v += g.g_top[row * top + i];
-    d[j] = from_f32<T>(v);
-}
-
 __device__ __forceinline__ uint32_t class_or_none(long long j, int C) { return j >= 0 && j < C ? (uint32_t)j : 0xFFFFFFFFu; }
 // KMAX alternatives in registers, their places compared with every class.  More than 4 come through LDS, so that whole lines are read (as in the
 // forward kernel).  The next classes are on their way while these are stored: a store could alias them, so the compiler would not do it.
@@ -618,7 +594,8 @@ __global__ __launch_bounds__(256) void lp_lane_backward_kernel(const T* __restri
     }
 }
 
-// a block (NW = 4) or a wave (NW = 1) per part of a row; the alternatives' own terms are put right by the block that wrote them
+// a block (NW = 4) or a wave (NW = 1) per part of a row; the places of the target and of the alternatives get more than that, and are written again
+// by the first wave of the block that wrote them
 template <typename T, int NW>
 __global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int part_len,
                                                               Grad g, T* __restrict__ dx) {
@@ -629,7 +606,14 @@ __global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restric
     const T* p = x + row * row_stride;
     T* d = dx + row * C;
     const int lo = blockIdx.y * part_len, hi = C - lo < part_len ? C : lo + part_len;
-    const RowGrad r = row_grad(g, row, C, top_grads(g, row));
+    const int lane = threadIdx.x & 63, top = g.g_top ? g.top : 0;      // lane 1 + i has alternative i
+    const bool mine = lane > 0 && lane <= top;
+    const int at = mine ? (int)class_or_none(g.top_index[row * top + lane - 1], C) : -1;
+    const float b = mine ? g.g_top[row * top + lane - 1] : 0.f;
+    const RowGrad r = row_grad(g, row, C, top ? wave_sum(b) : 0.f);
+    const int j = lane ? at : r.t;
+    const bool here = lane <= top && j >= lo && j < hi;
+    const float xj = here ? to_f32(p[j]) : 0.f;
     auto take = [&](float (&v)[VEC]) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = class_grad(r, v[e]);
@@ -661,7 +645,14 @@ __global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restric
     // (behind the block's stores to these places)
     if constexpr (NW > 1) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-    place_grad<T>(r, g, row, t, lo, hi, p, d);
+    if (t > 63 || r.logs == INFINITY) return;
+    float v = class_grad(r, xj) + (j == r.t ? r.a : 0.f);
+    for (int i = 1; i <= top; ++i) {
+        const int ai = __builtin_amdgcn_readlane(at, i);
+        const float bi = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(b), i));
+        v += ai == j ? bi : 0.f;
+    }
+    if (here) d[j] = from_f32<T>(v);                                   // (the same place: the same value)
 }
 
 // few long rows: enough parts for about four blocks on every CU, none under 256 lanes' accesses of 16 bytes
