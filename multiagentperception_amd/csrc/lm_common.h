@@ -104,6 +104,16 @@ __device__ __forceinline__ u32x4_t load_raw_part(const T* __restrict__ p, long l
     for (int i = 0; i < VEC; ++i) t.v[i] = i < n ? p[i] : from_f32<T>(fill);
     return __builtin_bit_cast(u32x4_t, t);
 }
+// ... the elements [lo, hi) of an access that starts at c, before, in or behind them
+template <typename T>
+__device__ __forceinline__ u32x4_t load_raw_range(const T* __restrict__ p, int c, int lo, int hi, float fill) {
+    constexpr int VEC = ElemOf<T>::VEC;
+    if (c >= lo && c + VEC <= hi) return load_raw<T>(p + c);
+    Pack<T, VEC> t;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t.v[i] = c + i >= lo && c + i < hi ? p[c + i] : from_f32<T>(fill);
+    return __builtin_bit_cast(u32x4_t, t);
+}
 template <typename T>
 __device__ __forceinline__ void widen(u32x4_t r, float (&v)[ElemOf<T>::VEC]) {
     const Pack<T, ElemOf<T>::VEC> t = __builtin_bit_cast(Pack<T, ElemOf<T>::VEC>, r);

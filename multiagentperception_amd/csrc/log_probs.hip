@@ -349,6 +349,28 @@ __device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int h
     return answer;
 }
 
+// The elements [lo, hi) of a row by a block's (or wave's) threads, groups of four accesses in flight; then each with f(raw, its first place).  Which accesses
+// there are goes by the row, not by the lane, so that the first and last ones, part of which is not there, cost no walk of their own.
+template <typename T, int NW, typename F>
+__device__ __forceinline__ void walk_row(const T* __restrict__ p, int origin, int lo, int hi, int t, float fill, F f) {
+    constexpr int EACH = NW * 64 * ElemOf<T>::VEC;
+    for (int g = origin; g < hi; g += 4 * EACH) {
+        const bool whole = g >= lo && hi - g >= 4 * EACH;
+        u32x4_t raw[4];
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[i] = load_raw<T>(p + g + i * EACH + t * ElemOf<T>::VEC);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (g + i * EACH < hi) raw[i] = load_raw_range<T>(p, g + i * EACH + t * ElemOf<T>::VEC, lo, hi, fill);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (whole || g + i * EACH < hi) f(raw[i], g + i * EACH + t * ElemOf<T>::VEC, whole);
+    }
+}
+
 // parts == nullptr: the whole row is here.  Otherwise part blockIdx.y of it, and its (m, s, u) and k keys go to parts / part_keys
 // [row][part] for lp_join_kernel.
 template <typename T, int NW>
@@ -365,40 +387,19 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
     const long long target = o.logp && !parts ? o.target[row] : -1;     // (here, not behind the sums: two trips to memory, one behind the other)
     const float xt = target >= 0 && target < C ? to_f32(p[target]) : 0.f;
     Run r{-INFINITY, 0.f, 0.f};
-    const int first = lo - misaligned(p + lo) + t * VEC;
+    const int origin = lo - misaligned(p + lo), first = origin + t * VEC;
     float best = -INFINITY;
     int at = first;                                      // the access that brought it first
-    auto take = [&](const float (&v)[VEC], int c) {
+    walk_row<T, NW>(p, origin, lo, hi, t, -INFINITY, [&](u32x4_t raw, int c, bool) {
+        float v[VEC];
+        widen<T>(raw, v);
         const float cm = max_of<VEC>(v);
         if (k) {
             at = cm > best ? c : at;
             best = __builtin_fmaxf(cm, best);
         }
         run_add<VEC>(r, v, cm);
-    };
-    int c = first;
-    if (c < lo) {
-        float v[VEC];
-        load_range<T, VEC>(p, c, lo, hi, v, -INFINITY);
-        take(v, c);
-        c += TPR * VEC;
-    }
-    for (; c + 3 * TPR * VEC + VEC <= hi; c += 4 * TPR * VEC) {          // four accesses in flight per lane
-        u32x4_t raw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = load_raw<T>(p + c + i * TPR * VEC);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v[VEC];
-            widen<T>(raw[i], v);
-            take(v, c + i * TPR * VEC);
-        }
-    }
-    for (; c < hi; c += TPR * VEC) {
-        float v[VEC];
-        load_range<T, VEC>(p, c, lo, hi, v, -INFINITY);
-        take(v, c);
-    }
+    });
     r = wave_join(r);
     if constexpr (NW > 1) {
         if ((threadIdx.x & 63) == 0) {
@@ -430,7 +431,7 @@ __global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict
     if (!k) return;
     key_t* mem = shared + (NW == 1 ? wave * top_keys_words<NW>(k) : 0);
     const key_t mine = first < hi ? key_of(best, at < lo ? lo : at) : 0;
-    const key_t q = top_keys<T, NW>(p, lo, hi, lo - misaligned(p + lo), mine, k, mem);
+    const key_t q = top_keys<T, NW>(p, lo, hi, origin, mine, k, mem);
     if (wave == 0 || NW == 1) {
         s.m = __shfl(s.m, 0, 64);
         s.logs = __shfl(s.logs, 0, 64);
@@ -614,34 +615,14 @@ __global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restric
     const int j = lane ? at : r.t;
     const bool here = lane <= top && j >= lo && j < hi;
     const float xj = here ? to_f32(p[j]) : 0.f;
-    auto take = [&](float (&v)[VEC]) {
+    walk_row<T, NW>(p, lo - misaligned(p + lo), lo, hi, t, 0.f, [&](u32x4_t raw, int c, bool whole) {
+        float v[VEC];
+        widen<T>(raw, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = class_grad(r, v[e]);
-    };
-    auto edge = [&](int c) {
-        float v[VEC];
-        load_range<T, VEC>(p, c, lo, hi, v, 0.f);
-        take(v);
-        store_range<T, VEC>(d, c, lo, hi, v);
-    };
-    int c = lo - misaligned(p + lo) + t * VEC;
-    if (c < lo) {
-        edge(c);
-        c += TPR * VEC;
-    }
-    for (; c + 3 * TPR * VEC + VEC <= hi; c += 4 * TPR * VEC) {          // four accesses in flight per lane
-        u32x4_t raw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = load_raw<T>(p + c + i * TPR * VEC);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v[VEC];
-            widen<T>(raw[i], v);
-            take(v);
-            store_n<T, VEC>(d + c + i * TPR * VEC, v);
-        }
-    }
-    for (; c < hi; c += TPR * VEC) edge(c);
+        if (whole) store_n<T, VEC>(d + c, v);
+        else store_range<T, VEC>(d, c, lo, hi, v);
+    });
     // (behind the block's stores to these places)
     if constexpr (NW > 1) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
