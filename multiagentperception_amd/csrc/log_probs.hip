@@ -10,7 +10,7 @@
 //
 // HBM-bound: one read forward, one read and one write backward.  Three shapes of work:
 //   lane per row   class dimension strided (label maps) or at most 64 classes: 64 neighbouring rows per wave, alternatives in registers
-//   wave per row   up to 2 048 contiguous classes
+//   wave per row   up to 2 048 contiguous classes; a wave for up to four rows that fit its registers (about 500 classes)
 //   block per row or per part of a row   longer; few long rows are split over blocks and joined by a second launch
 // Alternatives of the last two: every thread keeps the largest (value, index) of what it read; the k-th largest of those is a bound that
 // at most k threads reach, and only their values are looked through again.
@@ -68,9 +68,8 @@ __device__ __forceinline__ Run wave_join(Run r) {
 // order of the alternatives: larger value first, then lower index; NaN ranks as -inf.  0 = none
 typedef unsigned long long key_t;
 __device__ __forceinline__ uint32_t ordered(float v) {               // not below 2^22: -inf is 0x007FFFFF
-    const uint32_t b = __float_as_uint(v == v ? v : -INFINITY);
-    const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return v == 0.f ? 0x80000000u : o;                               // -0 and +0 are one value
+    const uint32_t b = __float_as_uint(__builtin_fmaxf(v, -INFINITY) + 0.f);               // NaN to -inf, -0 to +0
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
 __device__ __forceinline__ key_t key_of(float v, int index) { return (key_t)ordered(v) << 32 | (uint32_t)~index; }
@@ -90,6 +89,14 @@ __device__ __forceinline__ key_t wave_max_key(key_t k) {
                                              : (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, __builtin_ctzll(have));
     return (key_t)best << 32 | index;
 }
+
+// bf16 and f16 values leave 13 bits of an ordered f32 unused, and the class fits there where there are at most 8 192
+constexpr int LP_PACKED_CLASSES = 8192;
+constexpr uint32_t LP_PACKED = LP_PACKED_CLASSES - 1;
+__device__ __forceinline__ uint32_t packed_key(float v, int index) { return (ordered(v) & ~LP_PACKED) | (~(uint32_t)index & LP_PACKED); }
+__device__ __forceinline__ int key_index(uint32_t k) { return (int)(LP_PACKED - (k & LP_PACKED)); }
+__device__ __forceinline__ float key_value(uint32_t k) { return unordered(k & 0x80000000u ? k & ~LP_PACKED : k | LP_PACKED); }
+__device__ __forceinline__ uint32_t wave_max_key(uint32_t k) { return wave_max_bits(k); }
 
 struct Out {                                  // where a row's answers go
     const long long* target;
@@ -115,10 +122,8 @@ __device__ __forceinline__ Stat row_answer(const Run& r, const Out& o, long long
 
 // ---- lane per row ------------------------------------------------------------------------------------------------------------------------
 // The K largest of the classes a lane has walked, largest first; classes come in ascending order, so an equal one goes behind those before it.  A new
-// value x moves place k to the middle one of (place k - 1, x, place k): no chain from place to place.  bf16 and f16 values leave 13 bits of an
-// ordered f32 unused, and the class fits there (at most 8 192 of them): two instructions a place where f32 values take five.
-// 64 maps of 19 x 128 x 256, bf16 / f32, with 2, 5 and 16 alternatives: 51 / 53, 78 / 100 and 178 / 270 us (without any 36 / 41).
-constexpr int LP_LANE_CLASSES = 8192;
+// value x moves place k to the middle one of (place k - 1, x, place k): no chain from place to place, and two instructions a place for packed keys where
+// f32 values take five.  64 maps of 19 x 128 x 256, bf16 / f32, with 2, 5 and 16 alternatives: 46 / 52, 71 / 89 and 172 / 259 us (without any 31 / 39).
 template <typename T, int K>
 struct Largest {
     static constexpr bool ONE = sizeof(T) == 2;
@@ -132,25 +137,23 @@ struct Largest {
         }
     }
     __device__ __forceinline__ void add(float value, int j, bool there) {
-        uint32_t x = ordered(value);
-        if constexpr (ONE) x = (x & ~(uint32_t)(LP_LANE_CLASSES - 1)) | (uint32_t)(LP_LANE_CLASSES - 1 - j);
-        x = there ? x : 0;
+        const uint32_t x = !there ? 0 : ONE ? packed_key(value, j) : ordered(value);
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) {
             if constexpr (!ONE) {
-                const int moved = k && x > v[k ? k - 1 : 0] ? at[k ? k - 1 : 0] : j;
-                at[k] = x > v[k] ? moved : at[k];
+                const int moved = k && x > v[k ? k - 1 : 0] ? +at[k ? k - 1 : 0] : j;
+                at[k] = x > v[k] ? +moved : +at[k];
             }
-            const uint32_t low = k && v[k ? k - 1 : 0] < x ? v[k ? k - 1 : 0] : x;
-            v[k] = low > v[k] ? low : v[k];
+            const uint32_t low = k && v[k ? k - 1 : 0] < x ? +v[k ? k - 1 : 0] : +x;
+            v[k] = low > v[k] ? +low : +v[k];
         }
     }
     __device__ __forceinline__ int index(int k) const {
-        if constexpr (ONE) return LP_LANE_CLASSES - 1 - (int)(v[k] & (LP_LANE_CLASSES - 1));
+        if constexpr (ONE) return key_index(v[k]);
         else return at[k];
     }
     __device__ __forceinline__ float value(int k) const {
-        if constexpr (ONE) return unordered(v[k] & 0x80000000u ? v[k] & ~(uint32_t)(LP_LANE_CLASSES - 1) : v[k] | (LP_LANE_CLASSES - 1));
+        if constexpr (ONE) return key_value(v[k]);
         else return unordered(v[k]);
     }
 };
@@ -221,6 +224,108 @@ __global__ __launch_bounds__(256) void lp_lane_forward_kernel(const T* __restric
             }
         }
     }
+}
+
+// ---- up to four short rows per wave ------------------------------------------------------------------------------------------------------
+template <typename K>
+__device__ __forceinline__ void order_pair(K& a, K& b) {
+    const K x = a, y = b;
+    a = x > y ? +x : +y;
+    b = x > y ? +y : +x;
+}
+template <typename K>
+__device__ __forceinline__ void sort_down(K (&k)[4]) {
+    order_pair(k[0], k[1]), order_pair(k[2], k[3]), order_pair(k[0], k[2]), order_pair(k[1], k[3]), order_pair(k[1], k[2]);
+}
+template <typename K>
+__device__ __forceinline__ void sort_down(K (&k)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) order_pair(k[i], k[i + 1]), order_pair(k[i + 2], k[i + 3]), order_pair(k[i], k[i + 2]), order_pair(k[i + 1], k[i + 3]), order_pair(k[i + 1], k[i + 2]);
+    order_pair(k[0], k[4]), order_pair(k[1], k[5]), order_pair(k[2], k[6]), order_pair(k[3], k[7]);
+    order_pair(k[2], k[4]), order_pair(k[3], k[5]), order_pair(k[1], k[2]), order_pair(k[3], k[4]), order_pair(k[5], k[6]);
+}
+// Rows of at most A accesses of 16 bytes a lane stay in registers, and `per` of them (up to four) share a wave: their loads are in flight together, and the
+// closing arithmetic of each is done by a lane of its own, at once.  Alternatives: every lane sorts its values, the largest of the lanes' first ones is
+// taken k times.  Bound by instructions: 65536 x 500 bf16 without alternatives, with 2, 8 and 20:
+// 26, 44, 54 and 79 us, where a wave per row that is walked like longer ones takes 32, 63, 83 and 124.
+template <typename T, int A>
+__global__ __launch_bounds__(256) void lp_short_forward_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int per, Out o) {
+    constexpr int VEC = ElemOf<T>::VEC, E = A * VEC, RW = 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = o.top;
+    const long long row0 = ((long long)blockIdx.x * 4 + wave) * per, row = row0 + lane;
+    if (row0 >= rows) return;                            // whole waves
+    const int n = rows - row0 < per ? (int)(rows - row0) : per;
+    u32x4_t raw[RW][A];
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+        if (r < n) {
+            const T* p = x + (row0 + r) * row_stride;
+#pragma unroll
+            for (int a = 0; a < A; ++a) raw[r][a] = load_raw_range<T>(p, (a * 64 + lane) * VEC - misaligned(p), 0, C, -INFINITY);
+        }
+    const long long target = lane < n && o.logp ? o.target[row] : -1;
+    const float xt = target >= 0 && target < C ? to_f32(x[row * row_stride + target]) : 0.f;
+    auto values = [&](int r, float (&v)[E]) {
+#pragma unroll
+        for (int a = 0; a < A; ++a) {
+            float w[VEC];
+            widen<T>(raw[r][a], w);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[a * VEC + e] = w[e];
+        }
+    };
+    Run mine{0.f, 1.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+        if (r < n) {
+            float v[E], s = 0.f, u = 0.f;
+            values(r, v);
+            const float m = wave_max(max_of<E>(v)), base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = v[e] - base, f = exp_d(d);
+                s += f;
+                u = fmaf(f, __builtin_fmaxf(d, LP_FLOOR), u);
+            }
+            s = wave_sum(s);
+            u = wave_sum(u);
+            if (lane == r) mine = Run{m, s, u};
+        }
+    Stat st{0.f, 0.f};
+    if (lane < n) st = row_answer(mine, o, row, C, target, xt);
+    if (!k) return;
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+        if (r < n) {
+            typedef std::conditional_t<sizeof(T) == 2, uint32_t, key_t> K;
+            const T* p = x + (row0 + r) * row_stride;
+            float v[E];
+            K key[E], answer = 0;
+            values(r, v);
+#pragma unroll
+            for (int a = 0; a < A; ++a)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {          // (what is absent is -inf and ranks behind what is there: places from C on, and below 0 as if from above)
+                    const int c = (a * 64 + lane) * VEC - misaligned(p) + e;
+                    if constexpr (sizeof(T) == 2) key[a * VEC + e] = packed_key(v[a * VEC + e], c);
+                    else key[a * VEC + e] = key_of(v[a * VEC + e], c);
+                }
+            sort_down(key);
+            for (int i = 0; i < k; ++i) {
+                const K best = wave_max_key(key[0]);
+                if (lane == i) answer = best;
+                uint32_t taken = key[0] == best ? ~0u : 0u;           // (bits: of a condition the compiler makes a choice of the index)
+                asm volatile("" : "+v"(taken));
+                const K move = sizeof(K) == 8 ? (K)((key_t)taken << 32 | taken) : (K)taken;
+#pragma unroll
+                for (int e = 0; e < E; ++e) key[e] = (move & (e + 1 < E ? +key[e + 1 < E ? e + 1 : e] : K(0))) | (~move & key[e]);
+            }
+            const float m = __shfl(st.m, r, 64), logs = __shfl(st.logs, r, 64);
+            if (lane < k) {
+                o.top_logp[(row0 + r) * k + lane] = (key_value(answer) - m) - logs;
+                o.top_index[(row0 + r) * k + lane] = key_index(answer);
+            }
+        }
 }
 
 // ---- wave or block per (part of a) row -----------------------------------------------------------------------------------------------------
@@ -679,6 +784,16 @@ int lp_forward(const void* x, long long outer, int C, long long inner, long long
         return w2c_launch_status();
     }
     const int k = o.top;
+    constexpr int VEC = ElemOf<T>::VEC, MOST = 8 / VEC;                  // eight values a lane
+    if (C + VEC - 1 <= 64 * VEC * MOST) {
+        const int per = outer >= 4 * 4096 ? 4 : outer >= 4096 ? 2 : 1;   // as many waves as the card holds before rows share one
+        const dim3 grid((unsigned)((outer + 4 * per - 1) / (4 * per)));
+        if (C + VEC - 1 <= 64 * VEC)
+            hipLaunchKernelGGL((lp_short_forward_kernel<T, 1>), grid, dim3(256), 0, st, (const T*)x, outer, C, row_stride, per, o);
+        else
+            hipLaunchKernelGGL((lp_short_forward_kernel<T, MOST>), grid, dim3(256), 0, st, (const T*)x, outer, C, row_stride, per, o);
+        return w2c_launch_status();
+    }
     if (C <= LP_WAVE_MOST) {
         hipLaunchKernelGGL((lp_row_forward_kernel<T, 1>), dim3((unsigned)((outer + 3) / 4)), dim3(256), (size_t)(k ? 4 * top_keys_words<1>(k) * sizeof(key_t) : 0), st,
                            (const T*)x, outer, C, row_stride, C, o, (float*)nullptr, (key_t*)nullptr);
@@ -730,7 +845,7 @@ int lp_backward(const void* x, long long outer, int C, long long inner, long lon
 
 bool lp_shape_ok(int dtype, long long outer, int C, long long inner, long long row_stride) {
     return dtype >= W2C_F32 && dtype <= W2C_F16 && outer >= 1 && outer <= 0x7FFFFFFF && C >= 1 && C <= (1 << 28) && inner >= 1 &&
-           inner <= 0x7FFFFFFF && (inner == 1 || C <= LP_LANE_CLASSES) && (inner > 1 ? row_stride == (long long)C * inner : row_stride >= C);
+           inner <= 0x7FFFFFFF && (inner == 1 || C <= LP_PACKED_CLASSES) && (inner > 1 ? row_stride == (long long)C * inner : row_stride >= C);
 }
 
 }  // namespace

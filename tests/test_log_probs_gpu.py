@@ -100,6 +100,12 @@ def test_rows(outer, C, top, dtype):
     _check(outer, C, 1, dtype, top, seed=outer + C, masked=0.0 if outer % 2 else 0.3)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("outer,C,top", [(4099, 70, 3), (16389, 253, 8), (16386, 254, 20), (16387, 505, 0), (4097, 509, 32)])
+def test_many_short_rows(outer, C, top, dtype):
+    _check(outer, C, 1, dtype, top, seed=outer + C, masked=0.3)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("outer,C,inner,top", [(2, 11, 35, 2), (1, 2, 1000, 1), (3, 19, 3, 8), (2, 40, 130, 20), (1, 33, 70, 32), (2, 1100, 5, 3)])
 def test_class_dimension_in_front(outer, C, inner, top, dtype):
