@@ -552,7 +552,10 @@ int launch_tile(const Product& p, hipStream_t st) {
 
 long long tiles(int M, int N, int tm, int tn) { return (long long)((M + tm - 1) / tm) * ((N + tn - 1) / tn); }
 // What a product of the tile kernels is cut into: the largest tiles of which there are enough for the 256 CUs (a larger tile reads less per product),
-// and where there are not enough of the smallest, parts of the reduction, of at least four blocks of 128 each.
+// and where there are at most half as many of the smallest, parts of the reduction: about 256 in all, each long enough to be worth the sum of the
+// parts (8 blocks of 128; 16 with more than 64 tiles, which already draw most of what the L2s give).  To bf16, with 8 / as it is / with 24 blocks at least:
+// 256 x 256 x 4096 9.3 / 9.3 / 11.2 us, 64 x 4096 x 4096 12.4 / 12.4 / 13.2, 1024 x 1024 x 2048 15.3 / 10.6 / 10.6; 512 parts instead of 256
+// take 1024 x 1024 x 4096 from 16.7 to 20.5 us and 512 x 512 x 8192 from 14.8 to 19.8.
 struct Cut {
     int tm, tn, parts;
 };
@@ -560,8 +563,8 @@ Cut product_cut(int M, int N, int K) {
     if (tiles(M, N, 256, 256) >= 160) return {256, 256, 1};
     if (tiles(M, N, 128, 128) >= 224) return {128, 128, 1};
     const long long t = tiles(M, N, 128, 64);
-    long long parts = t >= 192 ? 1 : 512 / t;
-    const int most = (K / KT + 3) / 4;
+    long long parts = t > 128 ? 1 : 256 / t;
+    const int least = t > 64 ? 16 : 8, most = (K / KT + least - 1) / least;
     if (parts > most) parts = most;
     if (parts > 16) parts = 16;
     return {128, 64, (int)parts};

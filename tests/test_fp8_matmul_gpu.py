@@ -126,6 +126,12 @@ def test_both_operands_with_tile_scales_and_a_long_reduction():
     _check(7, 200, 5000, b_tile=128, a_tile=128)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M,N,K", [(40, 100, 8192), (33, 65, 8200), (1000, 700, 4100), (1000, 700, 2000)])
+def test_a_long_reduction_in_parts(M, N, K, dtype):
+    _check(M, N, K, b_tile=128, dtype=dtype, bias=True)
+
+
 def test_a_nan_stays_in_its_row_or_column_and_a_scale_can_be_nan():
     a, b, _ = _operands(200, 300, 256, 1, 1)
     clean = ops.matmul_fp8(a, b, None, F32)
