@@ -2006,7 +2006,7 @@ def _rows(*columns):
 
 
 def _adamw_tensors(params, grads):
-    """(device, addresses of the parameters and of the gradients, elements, element types) after the checks of parameters and gradients.
+    """(device, addresses of the parameters and of the gradients, elements, element types, all contiguous) after the checks of both.
     (Attribute by attribute over whole lists: a step of a small network is bound by these checks.)"""
     n = len(params)
     if not n or len(grads) != n:
@@ -2019,11 +2019,12 @@ def _adamw_tensors(params, grads):
         raise W2CError("adamw: f32, bf16 or f16 parameters with gradients of their types expected")
     if set(map(_layout, grads)) != {torch.strided} or list(map(_shape, params)) != list(map(_shape, grads)) or {dev.index} != {*map(_index, params), *map(_index, grads)}:
         raise W2CError("adamw: dense gradients of the parameters' shapes on %s expected" % dev)
-    if not (all(map(_contiguous, params)) and all(map(_contiguous, grads))):
+    plain = all(map(_contiguous, params))
+    if not (plain and (grads is params or all(map(_contiguous, grads)))):
         for i, (p, g) in enumerate(zip(params, grads)):
             if not (p.is_contiguous() and g.is_contiguous()) and (p.stride() != g.stride() or not _dense(p)):
                 raise W2CError("adamw: parameter %d and its gradient must be laid out alike, without gaps" % i)
-    return dev, list(map(_ptr, params)), list(map(_ptr, grads)), list(map(_numel, params)), list(map(_ELEM.__getitem__, dtypes))
+    return dev, list(map(_ptr, params)), list(map(_ptr, grads)), list(map(_numel, params)), list(map(_ELEM.__getitem__, dtypes)), plain
 
 
 def _grad_squares(dev, rows, n):
@@ -2040,7 +2041,7 @@ def _grad_squares(dev, rows, n):
 
 def grad_squares(grads):
     """sums of the squares of parts of the gradients (f64), for adamw_step's `squares`: their total is the squared norm of all of them"""
-    dev, _, g, sizes, types = _adamw_tensors(grads, grads)
+    dev, _, g, sizes, types, _ = _adamw_tensors(grads, grads)
     none = [0] * len(g)
     return _grad_squares(dev, _rows(none, g, none, none, none, none, none, sizes, types), len(g))
 
@@ -2053,7 +2054,7 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
                                 scales of ADAMW_STATE_BLOCK elements; rounded at random by (seed, step, place)
     lr: a number, or an f32 device tensor of one element (a captured step then follows it).  max_norm: the gradients are scaled down to this
     norm in all; `squares` (grad_squares) where more tensors than these share the norm.  -> the norm before that (f32 on the device), or None."""
-    dev, p, g, sizes, types = _adamw_tensors(params, grads)
+    dev, p, g, sizes, types, plain = _adamw_tensors(params, grads)
     n = len(params)
     if len(states) != n or len(steps) != n or len({*map(len, states)}) != 1 or len(states[0]) not in (2, 4):
         raise W2CError("adamw: a step and a state, all (m, v) or all (m, m_scale, v, v_scale), for each of %d parameters expected" % n)
@@ -2066,7 +2067,7 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
         for t in parts:
             if {*map(_dtype, t)} != {torch.float32} or list(map(_numel, t)) != sizes:
                 raise W2CError("adamw: f32 moments of the parameters' elements expected")
-            if not (all(map(_contiguous, t)) and all(map(_contiguous, params))):
+            if not (plain and all(map(_contiguous, t))):
                 for i, (a, b) in enumerate(zip(params, t)):
                     if not (a.is_contiguous() and b.is_contiguous()) and a.stride() != b.stride():
                         raise W2CError("adamw: parameter %d: its moments must be laid out like it" % i)
