@@ -161,3 +161,27 @@ def test_two_streams_at_once():
         for a, b in zip(alone, got):
             for p, q in zip(a, b):
                 assert torch.equal(p, q)
+
+
+def test_calls_with_other_shapes_and_strides():
+    """single rows without a batch, classes in front, transposed and strided inputs, nothing at all: the same values as the stock operations'"""
+    torch.manual_seed(5)
+    head = Head().cuda()
+    v = torch.randn(77, device="cuda", requires_grad=True)
+    r = loss.log_probs(v, torch.tensor(5, device="cuda"), top=2)
+    (r.logp + r.entropy + r.top_logp.sum()).backward()
+    w = v.detach().double().cpu().requires_grad_()
+    lp = torch.log_softmax(w, 0)
+    (lp[5] - (lp.exp() * lp).sum() + lp.sort(descending=True)[0][:2].sum()).backward()
+    assert r.logp.shape == () and r.top_index.shape == (2,) and abs(float(r.logp.detach()) - float(lp[5].detach())) <= 80 * U * 10
+    assert (v.grad.double().cpu() - w.grad).abs().max() <= 400 * U * 4                 # terms up to 1 + 2 + the entropy's
+    m = torch.randn(9, 20, device="cuda", requires_grad=True)
+    front = loss.log_probs(m, torch.zeros(20, dtype=torch.long, device="cuda"), dim=0)
+    back = loss.log_probs(m.t(), torch.zeros(20, dtype=torch.long, device="cuda"))
+    assert (front.logp - back.logp).abs().max() <= 40 * U * 10 and (front.entropy - back.entropy).abs().max() <= 40 * U * 10
+    assert train_ops.layer_norm(torch.randn(33, device="cuda")).shape == (33,) and head.out(torch.randn(192, device="cuda")).shape == (300,)
+    t = torch.randn(192, 50, device="cuda").t()
+    assert torch.equal(head.norm(t), head.norm(t.contiguous())) and torch.equal(head.out(t), head.out(t.contiguous()))
+    e = loss.log_probs(torch.zeros(0, 7, device="cuda", requires_grad=True), torch.zeros(0, dtype=torch.long, device="cuda"), top=2)
+    e.logp.sum().backward()
+    assert e.top_index.shape == (0, 2) and e.entropy.shape == (0,)
