@@ -364,21 +364,22 @@ __device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int h
     }
     if (t == 0) counts[0] = counts[1] = 0;
     row_barrier<NW>();
-    if constexpr (NW > 1) {                              // every wave finds the k-th largest of all of them
+    if constexpr (NW > 1) {                              // the k-th largest of all of them
         static_assert(NW == 4 && LP_TOP_MOST <= 32, "two keys a lane");
-        key_t a = lane < NW * k ? firsts[lane] : 0, b = lane + 64 < NW * k ? firsts[lane + 64] : 0;
-        if (a < b) {
-            const key_t c = a;
-            a = b;
-            b = c;
-        }
-        for (int r = 0; r < k; ++r) {
-            bound = wave_max_key(a);
-            if (a == bound) {
-                a = b;
-                b = 0;
+        if (wave == 0) {
+            key_t a = lane < NW * k ? firsts[lane] : 0, b = lane + 64 < NW * k ? firsts[lane + 64] : 0;
+            order_pair(a, b);
+            for (int r = 0; r < k; ++r) {
+                bound = wave_max_key(a);
+                if (a == bound) {
+                    a = b;
+                    b = 0;
+                }
             }
+            if (lane == 0) firsts[0] = bound;            // (read by this wave only, above)
         }
+        __syncthreads();
+        bound = firsts[0];
     }
     const bool again = mine && mine >= bound;            // at most k threads
     if (again) chosen[atomicAdd(&counts[0], 1)] = t;
@@ -404,11 +405,7 @@ __device__ __forceinline__ key_t top_keys(const T* __restrict__ p, int lo, int h
     if (found <= LP_CANDIDATES) {
         if (wave == 0) {
             key_t a = lane < found ? lists[lane] : 0, b = lane + 64 < found ? lists[lane + 64] : 0;
-            if (a < b) {
-                const key_t c = a;
-                a = b;
-                b = c;
-            }
+            order_pair(a, b);
             for (int r = 0; r < k; ++r) {
                 const key_t best = wave_max_key(a);
                 if (lane == r) answer = best;
