@@ -5,7 +5,7 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)            in f32, rounded once to p's type
 //
 // HBM-bound: f32 parameters move 28 bytes an element with 32-bit moments, 16 with 8-bit ones.  Tensors travel as tables in the kernel
-// arguments (48 a launch), so nothing is copied to the device, nothing is kept between calls and a captured step replays as it is; a
+// arguments (60 to 190 a launch), so nothing is copied to the device, nothing is kept between calls and a captured step replays as it is; a
 // block finds its tensor by bisecting the table's prefix of chunks.  The step counters live on the device: one small launch advances them and
 // leaves each tensor's factors for the launches behind it.
 //
@@ -18,25 +18,30 @@
 
 namespace {
 
-constexpr int AW_TENSORS = 48;            // a launch's table: 48 x 64 bytes of the 4 KiB that kernel arguments may take
+// tensors of a launch's table, by the 4 KiB that kernel arguments may take: 48 bytes a tensor with 32-bit moments, 64 with 8-bit ones, 20 for the norm
+constexpr int AW_TENSORS32 = 80, AW_TENSORS8 = 60, SQ_TENSORS = 190;
 constexpr int AW_STEPS = 256;             // step counters per launch
 constexpr int AW_STATE = 256;             // elements per 8-bit scale
 constexpr int AW_FIELDS = 9;              // of a tensor's row in the C ABI: p, g, m, v, m_scale, v_scale, step, n, dtype
 constexpr int AW_CHUNK = 4096;            // elements per block
 constexpr int SQ_CHUNK = 16384, SQ_MOST = 1024;
 
-struct Table {
-    void* p[AW_TENSORS];
-    const void* g[AW_TENSORS];
-    void* m[AW_TENSORS];
-    void* v[AW_TENSORS];
-    uint8_t* ms[AW_TENSORS];
-    uint8_t* vs[AW_TENSORS];
-    long long n[AW_TENSORS];
-    int first[AW_TENSORS];                // the tensor's first block in this launch
-    int factors[AW_TENSORS];              // its row of factors
+template <int TENSORS>
+struct Table32 {
+    void* p[TENSORS];
+    const void* g[TENSORS];
+    void* m[TENSORS];
+    void* v[TENSORS];
+    long long n[TENSORS];
+    int first[TENSORS];                   // the tensor's first block in this launch
+    int factors[TENSORS];                 // its row of factors
     int tensors;
 };
+struct Table8 : Table32<AW_TENSORS8> {
+    uint8_t* ms[AW_TENSORS8];
+    uint8_t* vs[AW_TENSORS8];
+};
+static_assert(sizeof(Table32<AW_TENSORS32>) <= 4000 && sizeof(Table8) <= 4000, "a table and the other arguments");
 struct Factors {                          // of one tensor in this step
     float step_size, root_scale, decay, clip;
     uint32_t key, pad[3];
@@ -102,7 +107,7 @@ __device__ __forceinline__ void adamw_element(const Rates& k, const Factors& f, 
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void adamw32_kernel(Table t, const Factors* __restrict__ factors, Rates k) {
+__global__ __launch_bounds__(256) void adamw32_kernel(Table32<AW_TENSORS32> t, const Factors* __restrict__ factors, Rates k) {
     constexpr int VEC = ElemOf<T>::VEC;
     const int i = find_tensor(t.first, t.tensors, blockIdx.x);
     const long long base = (long long)(blockIdx.x - t.first[i]) * AW_CHUNK, n = t.n[i];
@@ -228,7 +233,7 @@ __device__ __forceinline__ void adamw8_block(const Factors& f, const Rates& k, T
 
 // a wave per block of 256; nothing is shared between waves
 template <typename T>
-__global__ __launch_bounds__(256) void adamw8_kernel(Table t, const Factors* __restrict__ factors, Rates k) {
+__global__ __launch_bounds__(256) void adamw8_kernel(Table8 t, const Factors* __restrict__ factors, Rates k) {
     const int i = find_tensor(t.first, t.tensors, blockIdx.x);
     const long long n = t.n[i];
     const Factors f = factors[t.factors[i]];
@@ -246,11 +251,12 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Table t, const Factors* __r
 }
 
 struct SquareTable {
-    const void* g[AW_TENSORS];
-    long long n[AW_TENSORS];
-    int first[AW_TENSORS];                // the tensor's first chunk of SQ_CHUNK
+    const void* g[SQ_TENSORS];
+    long long n[SQ_TENSORS];
+    int first[SQ_TENSORS];                // the tensor's first chunk of SQ_CHUNK
     int tensors, chunks;
 };
+static_assert(sizeof(SquareTable) <= 4000, "a table and the other arguments");
 // a block's sum of squares over every gridDim.x-th chunk, in 64 bits (an f32 square overflows at 1.8e19)
 template <typename T>
 __global__ __launch_bounds__(256) void grad_squares_kernel(SquareTable t, double* __restrict__ out) {
@@ -287,16 +293,16 @@ bool aw_rows_ok(const long long* tensors, int n) {
     return true;
 }
 
-// walks the tensors of one element type in launches of at most AW_TENSORS tensors and 2^30 blocks; add(row, index, first block, blocks), flush(blocks)
+// walks the tensors of one element type in launches of at most `most` tensors and 2^30 blocks; add(row, index, first block, blocks), flush(blocks)
 template <typename Add, typename Flush>
-bool aw_batches(const long long* tensors, int n, int dtype, long long chunk, Add add, Flush flush) {
+bool aw_batches(const long long* tensors, int n, int dtype, int most, long long chunk, Add add, Flush flush) {
     int count = 0;
     long long blocks = 0;
     for (int i = 0; i < n; ++i) {
         const long long* r = row(tensors, i);
         if (r[8] != dtype || r[7] == 0) continue;
         const long long need = (r[7] + chunk - 1) / chunk;
-        if (count && (count == AW_TENSORS || blocks + need > (1ll << 30))) {
+        if (count && (count == most || blocks + need > (1ll << 30))) {
             if (!flush(count, (int)blocks)) return false;
             count = 0;
             blocks = 0;
@@ -312,7 +318,7 @@ int squares_blocks(const long long* tensors, int n, double* out, hipStream_t st,
     for (int dtype = W2C_F32; dtype <= W2C_F16; ++dtype) {
         SquareTable t;
         aw_batches(
-            tensors, n, dtype, SQ_CHUNK,
+            tensors, n, dtype, SQ_TENSORS, SQ_CHUNK,
             [&](const long long* r, int, int at, int first) {
                 t.g[at] = (const void*)r[1];
                 t.n[at] = r[7];
@@ -376,38 +382,45 @@ extern "C" int w2c_adamw_step(const long long* tensors, int n, int state_bits, d
     }
     const Rates k{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
     int status = W2C_OK;
-    for (int dtype = W2C_F32; dtype <= W2C_F16; ++dtype) {
-        Table t;
-        aw_batches(
-            tensors, n, dtype, AW_CHUNK,
-            [&](const long long* r, int i, int at, int first) {
-                t.p[at] = (void*)r[0];
-                t.g[at] = (const void*)r[1];
-                t.m[at] = (void*)r[2];
-                t.v[at] = (void*)r[3];
-                t.ms[at] = (uint8_t*)r[4];
-                t.vs[at] = (uint8_t*)r[5];
-                t.n[at] = r[7];
-                t.first[at] = first;
-                t.factors[at] = i;
-            },
-            [&](int count, int blocks) {
-                t.tensors = count;
+    auto fill = [](auto& t, const long long* r, int i, int at, int first) {
+        t.p[at] = (void*)r[0];
+        t.g[at] = (const void*)r[1];
+        t.m[at] = (void*)r[2];
+        t.v[at] = (void*)r[3];
+        t.n[at] = r[7];
+        t.first[at] = first;
+        t.factors[at] = i;
+    };
 #define AW_LAUNCH(KERNEL, T) hipLaunchKernelGGL((KERNEL<T>), dim3(blocks), dim3(256), 0, st, t, (const Factors*)factors, k)
-                if (state_bits == 32) {
-                    if (dtype == W2C_F32) AW_LAUNCH(adamw32_kernel, float);
-                    else if (dtype == W2C_BF16) AW_LAUNCH(adamw32_kernel, bf16_t);
-                    else AW_LAUNCH(adamw32_kernel, f16_t);
-                } else {
-                    if (dtype == W2C_F32) AW_LAUNCH(adamw8_kernel, float);
-                    else if (dtype == W2C_BF16) AW_LAUNCH(adamw8_kernel, bf16_t);
-                    else AW_LAUNCH(adamw8_kernel, f16_t);
-                }
-#undef AW_LAUNCH
-                status = w2c_launch_status();
-                return status == W2C_OK;
-            });
+#define AW_FLUSH(KERNEL)                                      \
+    [&](int count, int blocks) {                              \
+        t.tensors = count;                                    \
+        if (dtype == W2C_F32) AW_LAUNCH(KERNEL, float);       \
+        else if (dtype == W2C_BF16) AW_LAUNCH(KERNEL, bf16_t); \
+        else AW_LAUNCH(KERNEL, f16_t);                        \
+        status = w2c_launch_status();                         \
+        return status == W2C_OK;                              \
+    }
+    for (int dtype = W2C_F32; dtype <= W2C_F16; ++dtype) {
+        if (state_bits == 32) {
+            Table32<AW_TENSORS32> t;
+            aw_batches(
+                tensors, n, dtype, AW_TENSORS32, AW_CHUNK, [&](const long long* r, int i, int at, int first) { fill(t, r, i, at, first); },
+                AW_FLUSH(adamw32_kernel));
+        } else {
+            Table8 t;
+            aw_batches(
+                tensors, n, dtype, AW_TENSORS8, AW_CHUNK,
+                [&](const long long* r, int i, int at, int first) {
+                    fill(t, r, i, at, first);
+                    t.ms[at] = (uint8_t*)r[4];
+                    t.vs[at] = (uint8_t*)r[5];
+                },
+                AW_FLUSH(adamw8_kernel));
+        }
         if (status != W2C_OK) return status;
     }
+#undef AW_FLUSH
+#undef AW_LAUNCH
     return W2C_OK;
 }

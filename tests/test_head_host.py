@@ -128,8 +128,8 @@ def test_adamw_step_refuses(lib, change):
 
 def test_grad_squares_counts_blocks_and_refuses(lib):
     assert lib.w2c_grad_squares_count(_rows(GOOD), 1) == 1 and lib.w2c_grad_squares_count(_rows(GOOD[:7] + [0, 0]), 1) == 0
-    many = _rows(*[GOOD[:7] + [1 << 20, k % 3] for k in range(200)])          # 64 chunks each; 67, 67 and 66 tensors of a type in launches of 48: at most 1 024 blocks a launch
-    assert lib.w2c_grad_squares_count(many, 200) == 3 * 1024 + 2 * 1024 + 1024
+    many = _rows(*[GOOD[:7] + [1 << 20, k % 3] for k in range(600)])          # 64 chunks each; 200 tensors of a type in launches of at most 190: at most 1 024 blocks a launch
+    assert lib.w2c_grad_squares_count(many, 600) == 3 * (1024 + 640)
     assert lib.w2c_grad_squares_count(0, 1) == -1 and lib.w2c_grad_squares(_rows(GOOD), 1, 0, 1, 0) == -1 and lib.w2c_grad_squares(_rows(GOOD), 1, P, 0, 0) == -1
 
 
