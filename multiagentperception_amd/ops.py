@@ -7,8 +7,8 @@ capturable in a graph).  There is no fallback: CPU tensors raise.
 """
 import array
 import contextlib
-import functools
 import itertools
+import math
 import operator
 import threading
 import typing
@@ -1792,6 +1792,11 @@ def _on(dev):
     return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
+def _new(dev, dtype, *shape):
+    """torch.empty, by its quicker signature (sizes as numbers, 1.3 us; as a tuple 1.6)"""
+    return torch.empty(*shape, dtype=dtype, device=dev) if shape else torch.empty((), dtype=dtype, device=dev)
+
+
 _ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # the C ABI's element types
 
 
@@ -1834,7 +1839,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None):
     rows = x.numel() // cols
     y = torch.empty_like(x)
     h = torch.empty_like(x) if residual is not None else x
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    mean = _new(dev, torch.float32, *x.shape[:-1])
     rstd = torch.empty_like(mean)
     if rows:
         with _on(dev):
@@ -1895,13 +1900,9 @@ def _class_rows(x, dim, what):
     if not -x.dim() <= dim < x.dim():
         raise W2CError("%s: dim %d of a %d-dimensional tensor" % (what, dim, x.dim()))
     dim %= x.dim()
-    rest = tuple(x.shape[:dim]) + tuple(x.shape[dim + 1:])
-    outer, inner = 1, 1
-    for n in x.shape[:dim]:
-        outer *= n
-    for n in x.shape[dim + 1:]:
-        inner *= n
-    classes = x.shape[dim]
+    shape = tuple(x.shape)
+    rest, classes = shape[:dim] + shape[dim + 1:], shape[dim]
+    outer, inner = math.prod(shape[:dim]), math.prod(shape[dim + 1:])
     if classes < 1:
         raise W2CError("%s: no classes along dim %d of %s" % (what, dim, tuple(x.shape)))
     if x.is_contiguous():
@@ -1932,11 +1933,10 @@ def log_probs_forward(logits, target=None, top=0, dim=-1, ignore_index=-100):
         raise W2CError("log_probs: top must lie in 0 .. min(classes, %d), got %d of %d classes" % (LOG_PROBS_TOP_MOST, top, classes))
     if inner > 1 and classes > _LOG_PROBS_INNER_MOST:
         return log_probs_forward(logits.movedim(dim, -1).contiguous(), target, top, -1, ignore_index)
-    new = functools.partial(torch.empty, device=dev)
-    entropy, stats = new(rest, dtype=torch.float32), new(rest + (2,), dtype=torch.float32)
+    entropy, stats = _new(dev, torch.float32, *rest), _new(dev, torch.float32, *rest, 2)
     logp = torch.empty_like(entropy) if target is not None else None
-    top_logp = new(rest + (top,), dtype=torch.float32) if top else None
-    top_index = new(rest + (top,), dtype=torch.int64) if top else None
+    top_logp = _new(dev, torch.float32, *rest, top) if top else None
+    top_index = _new(dev, torch.int64, *rest, top) if top else None
     if outer * inner:
         lib = _native.lib()
         nbytes = lib.w2c_log_probs_workspace_bytes(outer, classes, inner, top)
@@ -2133,8 +2133,8 @@ class Fp8Quantized(typing.NamedTuple):
 
 
 def _fp8_new(rows, cols, tile, dev):
-    codes = torch.empty((rows, -(-cols // FP8_BLOCK) * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=dev)
-    return Fp8Blocks(codes, torch.empty((-(-rows // tile), codes.shape[1] // FP8_BLOCK), dtype=torch.float8_e8m0fnu, device=dev), cols)
+    blocks = -(-cols // FP8_BLOCK)
+    return Fp8Blocks(_new(dev, torch.float8_e4m3fn, rows, blocks * FP8_BLOCK), _new(dev, torch.float8_e8m0fnu, -(-rows // tile), blocks), cols)
 
 
 def quantize_fp8(x, tile=1, rows=True, columns=False, sums=False):
@@ -2190,7 +2190,7 @@ def matmul_fp8(a, b, bias=None, out_dtype=BF16):
         raise W2CError("matmul_fp8: f32, bf16 or f16 output expected, got %s" % out_dtype)
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,)):
         raise W2CError("matmul_fp8: bias must be f32 [%d]" % N)
-    c = torch.empty((M, N), dtype=out_dtype, device=dev)
+    c = _new(dev, out_dtype, M, N)
     if M and N:
         lib = _native.lib()
         nbytes = lib.w2c_matmul_fp8_workspace_bytes(M, N, K)
