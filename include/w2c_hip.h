@@ -563,7 +563,7 @@ int w2c_matmul_fp8(const void* a, const void* a_scale, int a_tile, const void* b
  * with tile 128][ceil(cols / 128)]), of the transposed x (codes_t [cols, rows padded to 128], 16-byte aligned, scale_t alike), either NULL if not
  * wanted, from one read.  A scale is the smallest power of two with amax <= 448 * scale, amax over the block's finite values (1 for zeros);
  * codes round to nearest even; values that are not finite become NaN.  column_sums: f32 [cols] = sums of x over its rows, or NULL (with it:
- * workspace of w2c_quantize_fp8_workspace_bytes). */
+ * workspace of w2c_quantize_fp8_workspace_bytes, 0: none). */
 long long w2c_quantize_fp8_workspace_bytes(long long rows, long long cols);
 int w2c_quantize_fp8(const void* x, int dtype, long long rows, long long cols, long long stride, int tile, void* codes, void* scale, void* codes_t,
                      void* scale_t, float* column_sums, void* workspace, long long workspace_bytes, w2c_stream_t stream);

@@ -618,7 +618,7 @@ extern "C" int w2c_matmul_fp8(const void* a, const void* a_scale, int a_tile, co
 }
 
 extern "C" long long w2c_quantize_fp8_workspace_bytes(long long rows, long long cols) {
-    return rows < 1 || cols < 1 ? W2C_E_ARG : (rows + 127) / 128 * cols * (long long)sizeof(float);
+    return rows < 1 || cols < 1 ? W2C_E_ARG : rows <= 128 ? 0 : (rows + 127) / 128 * cols * (long long)sizeof(float);      // (one tile's sums are the sums)
 }
 
 extern "C" int w2c_quantize_fp8(const void* x, int dtype, long long rows, long long cols, long long stride, int tile, void* codes, void* scale,
@@ -626,15 +626,16 @@ extern "C" int w2c_quantize_fp8(const void* x, int dtype, long long rows, long l
     if (!x || dtype < W2C_F32 || dtype > W2C_F16 || rows < 1 || cols < 1 || stride < cols || (tile != 1 && tile != 128)) return W2C_E_ARG;
     if ((!codes && !codes_t && !column_sums) || (codes && !scale) || (codes_t && !scale_t) || rows > 65535ll * 128 || cols > (1ll << 31)) return W2C_E_ARG;
     if (codes_t && (reinterpret_cast<uintptr_t>(codes_t) & 15)) return W2C_E_ARG;
-    if (column_sums && (!workspace || workspace_bytes < w2c_quantize_fp8_workspace_bytes(rows, cols))) return W2C_E_ARG;
+    const bool parts = column_sums && w2c_quantize_fp8_workspace_bytes(rows, cols) > 0;
+    if (parts && (!workspace || workspace_bytes < w2c_quantize_fp8_workspace_bytes(rows, cols))) return W2C_E_ARG;
     w2c_clear_error();
     const hipStream_t st = (hipStream_t)stream;
-    const Quantize q{x, rows, cols, stride, tile, (u8*)codes, (u8*)scale, (u8*)codes_t, (u8*)scale_t, column_sums ? (float*)workspace : nullptr};
+    const Quantize q{x, rows, cols, stride, tile, (u8*)codes, (u8*)scale, (u8*)codes_t, (u8*)scale_t, parts ? (float*)workspace : column_sums};
     const dim3 grid((unsigned)((cols + 127) / 128), (unsigned)((rows + 127) / 128));
     if (dtype == W2C_F32) hipLaunchKernelGGL((quantize_kernel<float>), grid, dim3(256), 0, st, q);
     else if (dtype == W2C_BF16) hipLaunchKernelGGL((quantize_kernel<bf16_t>), grid, dim3(256), 0, st, q);
     else hipLaunchKernelGGL((quantize_kernel<f16_t>), grid, dim3(256), 0, st, q);
-    if (column_sums)
+    if (parts)
         hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, (const float*)workspace, (rows + 127) / 128, cols,
                            column_sums);
     return w2c_launch_status();

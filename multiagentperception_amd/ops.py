@@ -2160,7 +2160,7 @@ def quantize_fp8(x, tile=1, rows=True, columns=False, sums=False):
         return Fp8Quantized(by_rows, by_cols, total)
     lib = _native.lib()
     nbytes = lib.w2c_quantize_fp8_workspace_bytes(R, C) if sums else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if sums else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on(dev):
         check(lib.w2c_quantize_fp8(_p(x), code, R, C, x.stride(0) if R > 1 else C, tile, *((_p(by_rows.codes), _p(by_rows.scale)) if rows else (None, None)),
                                    *((_p(by_cols.codes), _p(by_cols.scale)) if columns else (None, None)), _p(total), _p(ws), nbytes, _stream(dev)),

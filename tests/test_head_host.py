@@ -145,7 +145,8 @@ def test_matmul_fp8_refuses(lib, change):
 @pytest.mark.parametrize("change", [dict(x=0), dict(dtype=3), dict(rows=0), dict(cols=0), dict(stride=9), dict(tile=2), dict(codes=0, codes_t=0, sums=0), dict(scale=0), dict(scale_t=0),
                                     dict(rows=65535 * 128 + 1), dict(codes_t=P + 8), dict(ws=0), dict(nbytes=1)])
 def test_quantize_fp8_refuses(lib, change):
-    a = dict(x=P, dtype=0, rows=10, cols=10, stride=10, tile=1, codes=P, scale=P, codes_t=P, scale_t=P, sums=P, ws=P, nbytes=lib.w2c_quantize_fp8_workspace_bytes(10, 10))
+    assert lib.w2c_quantize_fp8_workspace_bytes(128, 10) == 0 and lib.w2c_quantize_fp8_workspace_bytes(0, 10) == -1
+    a = dict(x=P, dtype=0, rows=200, cols=10, stride=10, tile=1, codes=P, scale=P, codes_t=P, scale_t=P, sums=P, ws=P, nbytes=lib.w2c_quantize_fp8_workspace_bytes(200, 10))
     a.update(change)
     assert lib.w2c_quantize_fp8(a["x"], a["dtype"], a["rows"], a["cols"], a["stride"], a["tile"], a["codes"], a["scale"], a["codes_t"], a["scale_t"], a["sums"], a["ws"],
                                 a["nbytes"], 0) == -1
