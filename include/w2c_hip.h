@@ -554,11 +554,17 @@ int w2c_adamw_step(const long long* tensors, int n, int state_bits, double lr, c
 
 /* 8-bit product with a power-of-two scale per 128 of the reduction: c[m][n] = sum_k a[m][k] 2^(sa - 127) b[n][k] 2^(sb - 127) (+ bias[n]), c [M, N] of
  * dtype.  a [M, K], b [N, K]: e4m3fn codes, rows padded with zero codes to K, a multiple of 128, 16-byte aligned; a_scale e8m0
- * [a_tile = 1: M | 128: ceil(M / 128)][K / 128], b_scale alike: a scale per row or per 128 rows.  f32 accumulation, deterministic.  workspace: w2c_matmul_fp8_workspace_bytes
- * (0: none), 16-byte aligned. */
+ * [a_tile = 1: M | 128: ceil(M / 128)][K / 128], b_scale alike: a scale per row or per 128 rows.  The products are exact and
+ * added in f32 (a code times its scale goes in as a bf16 number: infinite beyond f32's range, a multiple of 2^-133); deterministic.  workspace: w2c_matmul_fp8_workspace_bytes (0: none),
+ * 16-byte aligned.
+ * _fast: dtype 1 or 2 alone, up to twice the rate; of the products of 8 neighbouring k (which k are neighbours is not defined within a block of 128) no
+ * more than the 13 bits below the largest are kept.  About 1.5e-5 of the result's norm on normal data; at most 7 * 2^-13 of the sum of the
+ * products' magnitudes, so an element that cancels can lose all its digits. */
 long long w2c_matmul_fp8_workspace_bytes(int M, int N, int K);
 int w2c_matmul_fp8(const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
                    const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, w2c_stream_t stream);
+int w2c_matmul_fp8_fast(const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
+                        const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, w2c_stream_t stream);
 /* The codes and scales of x [rows, cols] (row stride `stride` elements): by rows (codes [rows, cols padded to 128], scale [rows, or ceil(rows / 128)
  * with tile 128][ceil(cols / 128)]), of the transposed x (codes_t [cols, rows padded to 128], 16-byte aligned, scale_t alike), either NULL if not
  * wanted, from one read.  A scale is the smallest power of two with amax <= 448 * scale, amax over the block's finite values (1 for zeros);

@@ -95,6 +95,7 @@ SIGNATURES = {
     "w2c_layer_norm_backward": [_vp, _vp, _vp, _i, _ll, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
     "w2c_matmul_fp8_workspace_bytes": [_i, _i, _i],
     "w2c_matmul_fp8": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _ll, _vp],
+    "w2c_matmul_fp8_fast": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _ll, _vp],
     "w2c_quantize_fp8_workspace_bytes": [_ll, _ll],
     "w2c_quantize_fp8": [_vp, _i, _ll, _ll, _ll, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
     "w2c_grad_squares_count": [_vp, _i],

@@ -3,14 +3,16 @@
 //   C[m][n] = sum_k  a[m][k] 2^ea(m, k / 128)  b[n][k] 2^eb(n, k / 128)  (+ bias[n])
 //
 // Rows are stored padded with zero codes to a multiple of 128.  A scale belongs to one row's 128 (activations, gradients) or to a 128 x 128 tile
-// (weights: the transposed weights then have the same codes and scales).  gfx950's scaled matrix instructions multiply by both e8m0 scales
-// themselves, so one f32 accumulator runs through the whole reduction and no vector instruction touches the products.  Within a block of 128
-// the order of k is free as long as both operands agree, since its scale is one.
+// (weights: the transposed weights then have the same codes and scales).  Within a block of 128 the order of k is free as long as both
+// operands agree, since its scale is one.
 //
-// The scaled instructions line the products of 8 neighbouring k up to the largest of them and keep 13 bits below it (measured: a product 2^-14 of the
-// largest is lost, in the next group of 8 it is not): about 1.5e-5 of the result's norm, far below a bf16 or f16 output's own rounding
-// but not below an f32 one's.  An f32 output therefore goes through the bf16 instructions, which keep 23: a code times its scale is a bf16
-// number exactly (one conversion instruction per pair does both), at half the rate.
+// Products are summed in 32 bits: a code times its scale is a bf16 number exactly (one conversion instruction per pair does both; beyond f32's range it is
+// infinite, below 2^-126 a multiple of 2^-133), and the bf16 matrix instructions add exact products of those to an f32 accumulator: 4e-8 of the
+// result's norm, 8192^3 to bf16 in 769 us = 1.43 PFLOP/s (FAST: 1.5e-5, 459 us).
+// FAST, for outputs of 16 bits and callers that ask for it, feeds the codes to gfx950's scaled matrix instructions, which multiply by both e8m0
+// scales themselves at twice the rate.  They line the products of 8 neighbouring k up to the largest of them and keep 13 bits below it (measured: a
+// product 2^-14 of the largest is lost, in the next group of 8 it is not).  On normal data that is about 1.5e-5 of the result's norm, and
+// an element whose sum cancels can lose all its digits.
 //
 //   tile kernels   at least 25 rows: TM x TN tiles, both operands by LDS-DMA into a ring of four stages of 64 k
 //   row kernel     up to 24 rows (tokens being decoded): bound by reading b once; no LDS for operands, the waves of a block split k
@@ -80,10 +82,10 @@ __device__ __forceinline__ void wait_pieces() {               // at most N of th
 // t + 4, into the buffer of stage t (its reads were done before the barrier at the top of step t).  So a stage has three steps to arrive, and neither
 // its arrival nor an LDS read stands between the matrix instructions of two steps.  The scales of a block of 128 come with its first stage, into a
 // dword of LDS per row: four blocks' together where rows of scales are whole dwords (every row is a cache line of its own to the address unit:
-// 8192^3 to bf16 523 us with a byte per block, 512 with a dword per four; f32 outputs, at half the rate, lose 4 % by the branch and do without).
+// 8192^3 FAST to bf16 523 us with a byte per block, 512 with a dword per four; the bf16 instructions, at half the rate, lose 4 % by the branch and do without).
 // Stage image: row r (64 bytes) at 64 r, its 16-byte chunk c in slot c ^ ((r >> 2) & 3): 16 neighbouring rows' same chunk then cover all 64 banks once.
 // A piece of LDS-DMA is 16 rows (64 lanes x 16 bytes, contiguous in LDS); the swizzle is in the source address.
-template <typename T, int TM, int TN, int WM, int WN>
+template <typename T, bool FAST, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p, int tiles_m, int tiles_n) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int NW = WM * WN, MI = TM / WM / 32, NI = TN / WN / 32, PA = TM / 16 / NW, PB = TN / 16 / NW, HALF = KT / 2;
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
         srd_s[i] = descriptor((of_a ? p.sa : p.sb) + (long long)first * KB, (unsigned)(count < TM + TN ? count : TM + TN) * (unsigned)KB);
         svoff[i] = (unsigned)(((row < last ? row : last) >> shift) - first) * (unsigned)KB;
     }
-    const bool packed = sizeof(T) == 2 && (KB & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.sa) | reinterpret_cast<uintptr_t>(p.sb)) & 3) == 0;
+    const bool packed = FAST && (KB & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.sa) | reinterpret_cast<uintptr_t>(p.sb)) & 3) == 0;
     // piece i of stage t: scales first (a stage pair's come with its even one), then a's rows, then b's.  Behind the last stage the last is sent
     // again, into buffers that nothing reads any more: every step then has the same pieces to wait for.
     auto send = [&](int t, int i, bool with_scales) {
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
         if (i < PA) dma16(dst + i * NW * 1024u, voff + i * vstep, srd_a, soff);
         else dma16(dst + TM * HALF + (i - PA) * NW * 1024u, voff + (i - PA) * vstep, srd_b, soff);
     };
-    constexpr int EACH = PA + PB, TWO = 2 * EACH + (sizeof(T) == 4 ? (TM + TN) / 64 / NW : 0);      // pieces of a stage, and what two neighbours have at least
+    constexpr int EACH = PA + PB, TWO = 2 * EACH + (FAST ? 0 : (TM + TN) / 64 / NW);      // pieces of a stage, and what two neighbours have at least
     const int wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
     // a lane's 32 bytes of a stage: chunks 2 lhi, 2 lhi + 1 of rows l31 of its fragments
     const int key = (l31 >> 2) & 3, s0 = (((2 * lhi) ^ key) << 4), s1 = (((2 * lhi + 1) ^ key) << 4);
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
     struct Operands {
         u32x4_t a[MI][2], b[NI][2];
     };
-    constexpr int READS = 2 * (MI + NI), SREADS = MI + NI, QUARTERS = sizeof(T) == 4 ? 4 : 1, MULTS = MI * NI * QUARTERS;
+    constexpr int READS = 2 * (MI + NI), SREADS = MI + NI, QUARTERS = FAST ? 1 : 4, MULTS = MI * NI * QUARTERS;
     auto read = [&](Operands& f, unsigned buf, int i) {       // one of READS: b's fragments first
         const int k = i >> 1, h = i & 1;
         if (k < NI) f.b[k][h] = *reinterpret_cast<const u32x4_t*>(rb + buf + (h ? s1 : s0) + k * 32 * HALF);
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
     auto read_scales = [&](Scales& x, int kb, int i) {
         const int* s = reinterpret_cast<const int*>(smem + SCALES + ((packed ? kb >> 2 : kb) & 1) * SBUF) + l31;
         int v = s[i < NI ? TM + wn + i * 32 : wm + (i - NI) * 32] >> (packed ? 8 * (kb & 3) : 0);      // the scaled instructions take the lowest byte,
-        if constexpr (sizeof(T) == 4) v = (v & 255) << 23;                                             // the conversion a float's exponent field
+        if constexpr (!FAST) v = (v & 255) << 23;                                                   // the conversion a float's exponent field
         if (i < NI) x.b[i] = v;
         else x.a[i - NI] = v;
     };
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     auto multiply = [&](const Operands& f, const Scales& x, int q, int i, int j) {
-        if constexpr (sizeof(T) == 4) {                       // 16 k: a quarter of the stage
+        if constexpr (!FAST) {                                // 16 k: a quarter of the stage
             const bf16x8_t fb = scaled8(f.b[j][q >> 1][2 * (q & 1)], f.b[j][q >> 1][2 * (q & 1) + 1], __int_as_float(x.b[j]));
             const bf16x8_t fa = scaled8(f.a[i][q >> 1][2 * (q & 1)], f.a[i][q >> 1][2 * (q & 1) + 1], __int_as_float(x.a[i]));
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb, fa, acc[i][j], 0, 0, 0);
@@ -180,8 +182,9 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void matmul_tile_kernel(Product p,
                                                                         x.b[j], 0, x.a[i]);
     };
     // step t: multiply `now`, read stage t + 1 into `next`, send stage t + 4.  Reads and pieces are spread between the matrix instructions: in one go they
-    // would hold up the only wave of the SIMD for as long as the LDS and the address unit take for all four waves' (8192^3 to bf16: 721 us against 603).
-    // What is left is bound by power: the same product of zeros takes 360 us, of random codes 515; matrix instructions alone reach 3.7 PFLOP/s on random codes.
+    // would hold up the only wave of the SIMD for as long as the LDS and the address unit take for all four waves' (8192^3 FAST to bf16: 721 us against 603).
+    // What is left of FAST is bound by power: the same product of zeros takes 360 us, of random codes 515; matrix instructions alone reach 3.7 PFLOP/s on
+    // random codes.
     auto step = [&](const Operands& now, Operands& next, const Scales& x, Scales& x_next, int t, bool second) {
         const unsigned buf = (unsigned)((t + 1) & 3) * STAGE;
         const int pieces = EACH + (second ? 0 : PS), reads = READS + (second ? SREADS : 0);
@@ -286,7 +289,7 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(Product p) {
 }
 
 // At most 16 MT rows of a against 16 rows of b per block; wave w takes its share of the k blocks, the partial tiles are added in wave order.
-template <typename T, int MT, int NW>
+template <typename T, bool FAST, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void matmul_rows_kernel(Product p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ float part[NW][MT][256];
@@ -324,7 +327,7 @@ __global__ __launch_bounds__(NW * 64) void matmul_rows_kernel(Product p) {
             for (int t = 0; t < MT; ++t) {
                 const u8* q = pa[t] + (long long)(k0 + u) * KT;
                 const u32x4_t a0 = *reinterpret_cast<const u32x4_t*>(q), a1 = *reinterpret_cast<const u32x4_t*>(q + 64);
-                if constexpr (sizeof(T) == 4) {
+                if constexpr (!FAST) {
                     const float xa = __uint_as_float((sa[t] >> (8 * u) & 255u) << 23), xb = __uint_as_float((sb >> (8 * u) & 255u) << 23);
                     acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(scaled8(b0[u][0], b0[u][1], xb), scaled8(a0[0], a0[1], xa), acc[t], 0, 0, 0);
                     acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(scaled8(b0[u][2], b0[u][3], xb), scaled8(a0[2], a0[3], xa), acc[t], 0, 0, 0);
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
     }
 }
 
-template <typename T, int TM, int TN, int WM, int WN>
+template <typename T, bool FAST, int TM, int TN, int WM, int WN>
 int launch_tile(const Product& p, hipStream_t st) {
     const int tm = (p.M + TM - 1) / TM, tn = (p.N + TN - 1) / TN;
     constexpr int lds = 4 * (TM + TN) * (KT / 2) + 2 * (TM + TN) * 4;
@@ -539,12 +542,12 @@ int launch_tile(const Product& p, hipStream_t st) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return w2c_launch_status();
     if (!big[dev].load(std::memory_order_acquire)) {
-        if (hipFuncSetAttribute(reinterpret_cast<const void*>(&matmul_tile_kernel<T, TM, TN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, lds) !=
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(&matmul_tile_kernel<T, FAST, TM, TN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, lds) !=
             hipSuccess)
             return w2c_launch_status();
         big[dev].store(true, std::memory_order_release);
     }
-    hipLaunchKernelGGL((matmul_tile_kernel<T, TM, TN, WM, WN>), dim3(tm * tn, p.parts), dim3(WM * WN * 64), lds, st, p, tm, tn);
+    hipLaunchKernelGGL((matmul_tile_kernel<T, FAST, TM, TN, WM, WN>), dim3(tm * tn, p.parts), dim3(WM * WN * 64), lds, st, p, tm, tn);
     if (p.parts > 1)
         hipLaunchKernelGGL((sum_splits_kernel<T>), dim3((unsigned)(((long long)((p.N + 3) / 4) * p.M + 255) / 256)), dim3(256), 0, st, p);
     return w2c_launch_status();
@@ -570,7 +573,7 @@ Cut product_cut(int M, int N, int K) {
     return {128, 64, (int)parts};
 }
 
-template <typename T>
+template <typename T, bool FAST>
 int launch_product(const Product& p, hipStream_t st) {
     if (p.M <= ROWS_MOST) {
         const dim3 grid((p.N + 15) / 16);
@@ -578,8 +581,8 @@ int launch_product(const Product& p, hipStream_t st) {
         const bool few = p.N < 16 * 768 && p.K >= 16 * KT;
 #define MATMUL_ROWS(MT)                                                                                                             \
     do {                                                                                                                            \
-        if (few) hipLaunchKernelGGL((matmul_rows_kernel<T, MT, 16>), grid, dim3(1024), 0, st, p);                                    \
-        else hipLaunchKernelGGL((matmul_rows_kernel<T, MT, 4>), grid, dim3(256), 0, st, p);                                          \
+        if (few) hipLaunchKernelGGL((matmul_rows_kernel<T, FAST, MT, 16>), grid, dim3(1024), 0, st, p);                                    \
+        else hipLaunchKernelGGL((matmul_rows_kernel<T, FAST, MT, 4>), grid, dim3(256), 0, st, p);                                          \
     } while (0)
         if (p.M <= 16) MATMUL_ROWS(1);
         else MATMUL_ROWS(2);
@@ -587,34 +590,46 @@ int launch_product(const Product& p, hipStream_t st) {
         return w2c_launch_status();
     }
     const Cut cut = product_cut(p.M, p.N, p.K);
-    if (cut.tm == 256) return launch_tile<T, 256, 256, 2, 2>(p, st);
-    if (cut.tn == 128) return launch_tile<T, 128, 128, 2, 2>(p, st);
-    return launch_tile<T, 128, 64, 2, 2>(p, st);
+    if (cut.tm == 256) return launch_tile<T, FAST, 256, 256, 2, 2>(p, st);
+    if (cut.tn == 128) return launch_tile<T, FAST, 128, 128, 2, 2>(p, st);
+    return launch_tile<T, FAST, 128, 64, 2, 2>(p, st);
 }
 
-}  // namespace
-
-extern "C" long long w2c_matmul_fp8_workspace_bytes(int M, int N, int K) {
+long long workspace_bytes_of(int M, int N, int K) {
     if (M < 1 || N < 1 || K < KT || K % KT) return W2C_E_ARG;
     const int parts = M <= ROWS_MOST ? 1 : product_cut(M, N, K).parts;
     return parts > 1 ? (long long)parts * M * N * (long long)sizeof(float) : 0;
 }
 
-extern "C" int w2c_matmul_fp8(const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
-                              const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, void* stream) {
+int product(bool fast, const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
+            const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, void* stream) {
     if (!a || !a_scale || !b || !b_scale || !c || M < 1 || N < 1 || K < KT || K % KT || K > (1 << 22) || dtype < W2C_F32 || dtype > W2C_F16) return W2C_E_ARG;
     if ((a_tile != 1 && a_tile != 128) || (b_tile != 1 && b_tile != 128) || (long long)M * N > (1ll << 40)) return W2C_E_ARG;
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) return W2C_E_ARG;
     if ((long long)((M + 127) / 128) * ((N + 127) / 128) > 0x7FFFFFFF) return W2C_E_ARG;
     w2c_clear_error();
-    const long long need = w2c_matmul_fp8_workspace_bytes(M, N, K);
+    const long long need = workspace_bytes_of(M, N, K);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return W2C_E_ARG;
     const Product p{(const u8*)a, (const u8*)a_scale, (const u8*)b, (const u8*)b_scale, bias, c, M, N, K,
                     M <= ROWS_MOST ? 1 : product_cut(M, N, K).parts, (float*)workspace, a_tile == 128 ? 7 : 0, b_tile == 128 ? 7 : 0};
     const hipStream_t st = (hipStream_t)stream;
-    if (dtype == W2C_F32) return launch_product<float>(p, st);
-    if (dtype == W2C_BF16) return launch_product<bf16_t>(p, st);
-    return launch_product<f16_t>(p, st);
+    if (dtype == W2C_F32) return fast ? W2C_E_ARG : launch_product<float, false>(p, st);
+    if (dtype == W2C_BF16) return fast ? launch_product<bf16_t, true>(p, st) : launch_product<bf16_t, false>(p, st);
+    return fast ? launch_product<f16_t, true>(p, st) : launch_product<f16_t, false>(p, st);
+}
+
+}  // namespace
+
+extern "C" long long w2c_matmul_fp8_workspace_bytes(int M, int N, int K) { return workspace_bytes_of(M, N, K); }
+
+extern "C" int w2c_matmul_fp8(const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
+                              const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, void* stream) {
+    return product(false, a, a_scale, a_tile, b, b_scale, b_tile, M, N, K, bias, c, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int w2c_matmul_fp8_fast(const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
+                                   const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, void* stream) {
+    return product(true, a, a_scale, a_tile, b, b_scale, b_tile, M, N, K, bias, c, dtype, workspace, workspace_bytes, stream);
 }
 
 extern "C" long long w2c_quantize_fp8_workspace_bytes(long long rows, long long cols) {

@@ -2179,8 +2179,10 @@ def _fp8_tile(t, what):
     return 1 if scale.shape[0] == R else FP8_BLOCK
 
 
-def matmul_fp8(a, b, bias=None, out_dtype=BF16):
-    """a [M, K], b [N, K] (Fp8Blocks) -> a b^T (+ bias f32 [N]) as out_dtype [M, N]; f32 accumulation.  include/w2c_hip.h w2c_matmul_fp8."""
+def matmul_fp8(a, b, bias=None, out_dtype=BF16, fast=False):
+    """a [M, K], b [N, K] (Fp8Blocks) -> a b^T (+ bias f32 [N]) as out_dtype [M, N]; exact products, f32 accumulation.  fast: 16-bit outputs by the
+    8-bit matrix instructions, up to twice the rate; of 8 neighbouring products they keep no more than 13 bits below the largest (include/w2c_hip.h
+    w2c_matmul_fp8_fast: about 1.5e-5 of the result's norm, elements that cancel lose digits); an f32 output is the same with and without."""
     dev = _need_gpu(a.codes, a.scale, b.codes, b.scale, bias)
     ta, tb = _fp8_tile(a, "a"), _fp8_tile(b, "b")
     (M, K), (N, Kb) = a.codes.shape, b.codes.shape
@@ -2196,6 +2198,7 @@ def matmul_fp8(a, b, bias=None, out_dtype=BF16):
         nbytes = lib.w2c_matmul_fp8_workspace_bytes(M, N, K)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
         with _on(dev):
-            check(lib.w2c_matmul_fp8(_p(a.codes), _p(a.scale), ta, _p(b.codes), _p(b.scale), tb, M, N, K, _p(bias), _p(c), _ELEM[out_dtype],
-                                     _p(ws), nbytes, _stream(dev)), "w2c_matmul_fp8")
+            product = lib.w2c_matmul_fp8_fast if fast and out_dtype != torch.float32 else lib.w2c_matmul_fp8
+            check(product(_p(a.codes), _p(a.scale), ta, _p(b.codes), _p(b.scale), tb, M, N, K, _p(bias), _p(c), _ELEM[out_dtype], _p(ws), nbytes,
+                          _stream(dev)), "w2c_matmul_fp8")
     return c

@@ -395,12 +395,13 @@ class _LinearFp8Fn(torch.autograd.Function):
     is summed over, W with a scale per 128 x 128 tile.  Every operand is read once and quantised both ways from that read."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, fast):
         need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         rows = x.reshape(-1, x.shape[-1])
         xq = ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous(), 1, columns=need_w)
         wq = ops.quantize_fp8(weight.detach().contiguous(), ops.FP8_BLOCK, columns=need_x)
-        y = ops.matmul_fp8(xq.rows, wq.rows, None if bias is None else bias.detach().float().contiguous(), x.dtype)
+        y = ops.matmul_fp8(xq.rows, wq.rows, None if bias is None else bias.detach().float().contiguous(), x.dtype, fast)
+        ctx.fast = fast
         ctx.x_columns, ctx.w_columns = xq.columns, wq.columns
         ctx.shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
         return y.view(x.shape[:-1] + (weight.shape[0],))
@@ -408,26 +409,27 @@ class _LinearFp8Fn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         ops.first_order_only("linear_fp8")
-        need_x, need_w, need_b = ctx.needs_input_grad
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         rows = dy.reshape(-1, dy.shape[-1])
         q = ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous(), 1, rows=need_x, columns=need_w, sums=need_b)
         dx = dw = db = None
         if need_x:
-            dx = ops.matmul_fp8(q.rows, ctx.w_columns, None, ctx.dtypes[0]).view(ctx.shape)
+            dx = ops.matmul_fp8(q.rows, ctx.w_columns, None, ctx.dtypes[0], ctx.fast).view(ctx.shape)
         if need_w:
             if rows.shape[0]:
-                dw = ops.matmul_fp8(q.columns, ctx.x_columns, None, ctx.dtypes[1])
+                dw = ops.matmul_fp8(q.columns, ctx.x_columns, None, ctx.dtypes[1], ctx.fast)
             else:
                 dw = torch.zeros((dy.shape[-1], ctx.shape[-1]), dtype=ctx.dtypes[1], device=dy.device)
         if need_b:
             db = q.sums.to(ctx.dtypes[2])
-        return dx, dw, db
+        return dx, dw, db, None
 
 
-def linear_fp8(x, weight, bias=None):
-    """y [..., N] = x [..., K] W^T + bias with the product (and, under autograd, both products of its backward) in 8 bits with a power-of-two scale
-    per 128 elements of the sum.  weight: [N, K] f32 / bf16 / f16, or ops.Fp8Blocks of it (quantize_fp8(weight, 128).rows: laid out once, for
-    inference).  HIP kernels under the "hip" backend on GPU tensors, F.linear otherwise."""
+def linear_fp8(x, weight, bias=None, fast=False):
+    """y [..., N] = x [..., K] W^T + bias with the product (and, under autograd, both products of its backward) of 8-bit operands with a power-of-two
+    scale per 128 elements of the sum.  weight: [N, K] f32 / bf16 / f16, or ops.Fp8Blocks of it (quantize_fp8(weight, 128).rows: laid out once,
+    for inference).  fast: ops.matmul_fp8's, for the products with a 16-bit result (a gradient of f32 weights is not one).  HIP kernels under the
+    "hip" backend on GPU tensors, F.linear otherwise."""
     if isinstance(weight, ops.Fp8Blocks):
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise ops.W2CError("linear_fp8: quantised weights are for inference; pass the weights themselves to differentiate")
@@ -435,20 +437,24 @@ def linear_fp8(x, weight, bias=None):
             raise ops.W2CError("linear_fp8: %d features against weights of %d" % (x.shape[-1], weight.cols))
         rows = x.reshape(-1, x.shape[-1])
         y = ops.matmul_fp8(ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous()).rows, weight,
-                           None if bias is None else bias.detach().float().contiguous(), x.dtype)
+                           None if bias is None else bias.detach().float().contiguous(), x.dtype, fast)
         return y.view(x.shape[:-1] + (y.shape[1],))
     if _backend == "hip" and x.is_cuda:
         if weight.dim() != 2 or not weight.numel() or weight.shape[1] != x.shape[-1] or (bias is not None and tuple(bias.shape) != (weight.shape[0],)):
             raise ops.W2CError("linear_fp8: x %s, weight %s and bias do not fit" % (tuple(x.shape), tuple(weight.shape)))
-        return _LinearFp8Fn.apply(x, weight, bias)
+        return _LinearFp8Fn.apply(x, weight, bias, fast)
     return F.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
 
 
 class LinearFp8(nn.Linear):
-    """nn.Linear (same parameters, same state_dict keys) on linear_fp8()"""
+    """nn.Linear (same parameters, same state_dict keys) on linear_fp8(); `fast` is linear_fp8's"""
+
+    def __init__(self, in_features, out_features, bias=True, device=None, dtype=None, fast=False):
+        super().__init__(in_features, out_features, bias, device, dtype)
+        self.fast = fast
 
     def forward(self, x):
-        return linear_fp8(x, self.weight, self.bias)
+        return linear_fp8(x, self.weight, self.bias, self.fast)
 
 
 class GraphedTrainStep:
