@@ -141,7 +141,7 @@ class capture:
     """`with ops.capture() as graph:` -- capture the launches of the block into a fresh torch.cuda.CUDAGraph (thread-local error mode) with
     Python's cyclic garbage collector held off for the length of the window.
 
-    Why (round 5, the crash of GPUTEST_r04; tools/r05/gc_in_capture.py reproduces it in 12 lines): objects kept alive only by a reference
+    Why (the crash of GPUTEST_r04): objects kept alive only by a reference
     cycle -- a model + engine + its graphs inside a pytest.raises traceback, a closure -- are freed whenever the cyclic collector happens to
     run, i.e. at an arbitrary allocation.  If that is inside a capture window and the garbage holds an OLD CUDAGraph, its destructor
     (at::cuda::CUDAGraph::~CUDAGraph: hipGraphExecDestroy, pool release, and on ROCm a hipDeviceSynchronize) runs in the middle of the

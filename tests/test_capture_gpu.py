@@ -1,5 +1,5 @@
 """GPU: the capture window of this package (ops.capture) against Python's cyclic garbage collector -- the crash mechanism found behind
-GPUTEST_r04 (tools/r05/gc_in_capture.py, profiles/r05_capture_crash.txt): an OLD CUDAGraph kept alive only by a reference cycle is
+GPUTEST_r04 (profiles/r05_capture_crash.txt): an OLD CUDAGraph kept alive only by a reference cycle is
 finalised by whatever allocation triggers the collector; inside a capture window its destructor (hipDeviceSynchronize on ROCm) kills the
 process.  Each scenario runs in a subprocess so that a regression is an assertion, not a dead test session."""
 import os
@@ -44,15 +44,6 @@ if mode == "guarded":
     g2.replay(); torch.cuda.synchronize()
     assert float(z[0]) == 1.0
     print("GUARDED_OK")
-elif mode == "unguarded":
-    old_graph_garbage()
-    g2 = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g2, capture_error_mode="thread_local"):
-        z = x2 * 3
-        gc.collect()                          # what an unlucky allocation does
-        z = z + 1
-    g2.replay(); torch.cuda.synchronize()
-    print("UNGUARDED_SURVIVED")
 '''
 
 
@@ -65,13 +56,10 @@ def test_capture_window_holds_the_garbage_collector_off():
     assert r.returncode == 0 and "GUARDED_OK" in r.stdout, (r.returncode, r.stdout[-2000:], r.stderr[-4000:])
 
 
+@pytest.mark.skip(reason="made a GPU process abort on purpose (a CUDAGraph finalised inside a capture window); what it showed: profiles/r05_capture_crash.txt")
 def test_the_hazard_is_real_without_the_guard():
-    """Documents the mechanism on this stack (torch 2.10 / ROCm 7): the same sequence through a bare torch.cuda.graph dies (SIGABRT from
-    a check inside at::cuda::CUDAGraph::~CUDAGraph).  If a later stack survives it, the guard is merely unnecessary there: not a failure."""
-    r = _run("unguarded")
-    if r.returncode == 0:
-        pytest.skip("this stack tolerates a CUDAGraph finalised inside a capture window")
-    assert r.returncode < 0, (r.returncode, r.stderr[-2000:])
+    """The sequence of the test above through a bare torch.cuda.graph: SIGABRT from a check inside at::cuda::CUDAGraph::~CUDAGraph (torch 2.10 /
+    ROCm 7).  Not run any more, and without a body that could."""
 
 
 def test_no_capture_site_bypasses_the_guard():
@@ -88,7 +76,7 @@ def test_no_capture_site_bypasses_the_guard():
     assert hits and all(fn == "ops.py" for fn, _ in hits), hits
 
 
-def _repro(queues, script=("r05", "hipgraph_oob_repro.py"), args=("400", "3")):
+def _repro(queues, script, args):
     env = dict(os.environ)
     env.pop("GPU_MAX_HW_QUEUES", None)
     if queues is not None:
@@ -122,16 +110,10 @@ def test_the_package_sets_no_runtime_environment_variables():
     assert r.returncode == 0 and "ENV None None" in r.stdout, (r.stdout[-300:], r.stderr[-1500:])
 
 
-@pytest.mark.skipif(os.environ.get("W2C_RUN_RUNTIME_DEFECT_REPRO") != "1",
-                    reason="opt-in (W2C_RUN_RUNTIME_DEFECT_REPRO=1): triggers the runtime's out-of-bounds read on purpose and may wedge a shared GPU")
+@pytest.mark.skip(reason="made the runtime read out of bounds on purpose; what it showed: profiles/r05_capture_crash.txt")
 def test_the_runtime_defect_is_real_for_multi_branch_graphs_at_the_default_queue_count():
-    """Documents the defect on this stack: multi-branch graphs in pure torch at GPU_MAX_HW_QUEUES=4 (the runtime's default) die with SIGSEGV
-    inside libamdhip64's hipGraphLaunch within a few hundred launches (tools/r05/hipgraph_oob_repro.py).  A later runtime that survives makes
-    the single-branch design merely unnecessary, not wrong."""
-    r = _repro(4)
-    if r.returncode == 0:
-        pytest.skip("this HIP runtime survives the pattern at 4 hardware queues")
-    assert r.returncode < 0, (r.returncode, r.stderr[-1500:])
+    """Multi-branch graphs in pure torch at 4 hardware queues (the runtime's default): SIGSEGV inside libamdhip64's hipGraphLaunch within a few
+    hundred launches.  Not run any more, and without a body that could."""
 
 
 def test_recorded_program_equals_the_eager_run_and_consists_of_single_branch_graphs():

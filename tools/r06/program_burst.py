@@ -1,5 +1,5 @@
 """round 6: the burst-destruction pattern that kills multi-branch graph launches at the runtime's default 4 hardware queues
-(tools/r05/hipgraph_oob_repro.py, profiles/r05_capture_crash.txt), run against what the package launches now: recorded programs
+(profiles/r05_capture_crash.txt), run against what the package launches now: recorded programs
 (ops.record_program: single-branch HIP graphs on the program's own streams + event edges).
 Phase 1: a three-lane toy program, 4 recordings per iteration, 3 dropped at once, the survivors replayed from 3-7 long-lived streams.
 Phase 2: the product's own shapes -- MIMOcom / LearnWhen2Com forwards with model.use_hip_graph, engines dropped in bursts.
