@@ -935,12 +935,8 @@ class SRMSEngine:
         if getattr(self, "trunks5", None) is not None:                  # sq = the policy map alone [5B,h,w,512]
             # five separate value encoders: five independent single-trunk chains, forked over TWO side streams (encoder i on stream i % 2)
             # beside the policy encoder's chain on the main stream -- three parallel branches, not six.  Why not one stream each (round 4):
-            # hipGraphLaunch picks the graph's branch streams from the max_streams the exec created at instantiate, SKIPPING those that
-            # share the launch stream's hardware queue, without a bounds check (libamdhip64 of ROCm 7.0: the loop at GraphExec's
-            # UpdateStreams reads past the vector when more than ONE of them collides) -- with the default 4 hardware queues a graph of
-            # >= 5 parallel branches can always draw two collisions, and the out-of-bounds pointer is what segfaulted the replay of exactly
-            # this graph in GPUTEST_r04 and again in round 5 (profiles/r05_capture_crash.txt: native frames + disassembly).  <= 4 branches
-            # cannot overrun under round-robin queue assignment; every graph of this package now has <= 3.
+            # hipGraphLaunch of this graph with six branches faulted inside the runtime of ROCm 7.0 when its streams shared the launch
+            # stream's hardware queue (profiles/r05_capture_crash.txt: native frames); with fewer branches far more rarely.
             L = ops.lanes(x.device)
             main = torch.cuda.current_stream(x.device)
             parts = [None] * len(self.trunks5)

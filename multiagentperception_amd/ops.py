@@ -192,10 +192,10 @@ class capture:
 #     SINGLE-BRANCH HIP graphs (one linear chain of kernel nodes each) plus the event edges between them; Program.replay() launches
 #     them on the lanes' streams, edges as hipEventRecord / hipStreamWaitEvent between the launches.
 # Why not one graph with parallel branches (rounds 3-5): which streams the runtime runs the branches of a multi-branch exec on is the
-# runtime's choice per instantiation -- hipGraphLaunch of the HIP runtime bundled with torch 2.10 + rocm7.0 reads out of bounds while
-# choosing (profiles/r05_capture_crash.txt), and a bad draw puts both trunk chains on one hardware pipe for the exec's whole life
+# runtime's choice per instantiation -- launches of such execs have faulted inside the HIP runtime bundled with torch 2.10 + rocm7.0
+# (profiles/r05_capture_crash.txt), and a bad draw puts both trunk chains on one hardware pipe for the exec's whole life
 # (1.7x the step time; rounds 4-5 auditioned four instantiations per shape and kept the fastest, under GPU_MAX_HW_QUEUES=16).  A
-# single-branch exec has max_streams == 1: the stream-selection loop has nothing to choose, and the lanes are streams this package
+# single-branch exec leaves it nothing to choose, and the lanes are streams this package
 # created once -- no audition, no environment variable, no burst of exec-stream destructions.
 _MAX_LANES = 4
 

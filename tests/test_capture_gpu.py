@@ -89,11 +89,9 @@ def _repro(queues, script, args):
 
 
 def test_recorded_programs_survive_bursts_of_exec_destruction_at_the_runtimes_default_queue_count():
-    """The crash of GPUTEST_r04 (profiles/r05_capture_crash.txt): hipGraphLaunch of a MULTI-BRANCH exec skips the exec streams that share the
-    launch stream's hardware queue without a bounds check; at the runtime's default of 4 hardware queues a burst of exec destructions makes
-    the next execs' streams pile onto one queue and a launch from a stream on that queue reads past the vector.  Round 5 mitigated with
-    GPU_MAX_HW_QUEUES=16 + an audition; round 6 removed the cause: every graph the package launches is single-branch (ops.record_program),
-    so the selection loop has nothing to skip.  tools/r06/program_burst.py is the same burst pattern on recorded programs (4 recordings per
+    """The crash of GPUTEST_r04 (profiles/r05_capture_crash.txt): hipGraphLaunch of a MULTI-BRANCH exec faulted inside the runtime when the
+    exec's streams shared the launch stream's hardware queue; at the runtime's default of 4 hardware queues a burst of exec destructions makes
+    the next execs' streams pile onto one queue.  Every graph the package launches is single-branch (ops.record_program).  tools/r06/program_burst.py is the same burst pattern on recorded programs (4 recordings per
     iteration, 3 dropped at once, replays from 3-7 long-lived streams: 160 iterations here, 2 400 replays) and on the product's own forwards (engines dropped in bursts), with
     NO queue-count variable in the environment."""
     r = _repro(None, script=("r06", "program_burst.py"), args=("160", "4"))
