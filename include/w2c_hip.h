@@ -511,7 +511,8 @@ int w2c_nhwc_bf16_to_nchw_f32(const uint16_t* x, int x_cstride, int M, int C, in
  *   h = x + residual (rounded to dtype; residual NULL: h = x and `h` is not written), y = (h - mean) * rstd * weight + bias.
  * weight / bias: [cols] of wtype (0 = f32, or dtype) or NULL (1 / 0); mean, rstd: f32 [rows], for the backward.
  * backward: dx = gradient of x and of residual (dh: gradient that reaches h by another way, added; or NULL), dweight / dbias [cols] of wtype
- * (NULL: not wanted), workspace: w2c_layer_norm_workspace_bytes.  Deterministic (no atomics). */
+ * (NULL: not wanted), workspace: w2c_layer_norm_workspace_bytes.  Deterministic (no atomics).
+ * cols <= 2^30; rows < 2^31, with more than 16 384 columns < 2^22. */
 int w2c_layer_norm_forward(const void* x, const void* residual, int dtype, long long rows, int cols, const void* weight, const void* bias, int wtype,
                            float eps, void* y, void* h, float* mean, float* rstd, w2c_stream_t stream);
 long long w2c_layer_norm_workspace_bytes(long long rows, int cols, int dtype);
@@ -520,7 +521,7 @@ int w2c_layer_norm_backward(const void* dy, const void* h, const void* dh, int d
                             w2c_stream_t stream);
 
 /* Log probability of a given class, entropy and the `top` largest alternatives of every row of logits, one read of them.
- * x: [outer, classes, inner]; inner = 1: rows of `row_stride` >= classes elements; inner > 1: dense (row_stride = classes * inner), at most 8 192 classes.  Rows are
+ * x: [outer, classes, inner], outer and inner < 2^31, classes <= 2^28; inner = 1: rows of `row_stride` >= classes elements; inner > 1: dense (row_stride = classes * inner), at most 8 192 classes.  Rows are
  * numbered outer * inner.  target: int64 [rows] or NULL (then logp NULL); ignore_index there answers 0, any other value outside
  * [0, classes) NaN.  logp, entropy: f32 [rows]; top_logp f32, top_index int64 [rows, top], largest first, equal logits by the lower index
  * (top <= 32, <= classes; a NaN counts as -inf in this order); stats: f32 [rows, 2], for the backward.  -inf is a masked class; a row of nothing else
@@ -543,7 +544,7 @@ int w2c_log_probs_backward(const void* x, int dtype, long long outer, int classe
  * lr: lr_dev[0] (f32) where lr_dev is not NULL, so that a captured step follows it.  n_squares > 0: the gradients are scaled by
  * min(1, max_norm / (norm + 1e-6)), norm = sqrt(sum of squares), written to `norm` (f32 [1]) unless NULL; squares come from
  * w2c_grad_squares over all gradients that share the norm (same rows; only g, elements and dtype are read), w2c_grad_squares_count of them.
- * No row may share p, m, v or step with another.  workspace: w2c_adamw_workspace_bytes(n), 16-byte aligned, not shared with a call that
+ * No row may share p, m, v or step with another, and none has more than 2^36 - 4096 elements.  workspace: w2c_adamw_workspace_bytes(n), 16-byte aligned, not shared with a call that
  * may run at the same time.  Deterministic. */
 int w2c_grad_squares_count(const long long* tensors, int n);
 int w2c_grad_squares(const long long* tensors, int n, double* squares, int count, w2c_stream_t stream);

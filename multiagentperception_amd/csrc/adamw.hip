@@ -25,6 +25,7 @@ constexpr int AW_STATE = 256;             // elements per 8-bit scale
 constexpr int AW_FIELDS = 9;              // of a tensor's row in the C ABI: p, g, m, v, m_scale, v_scale, step, n, dtype
 constexpr int AW_CHUNK = 4096;            // elements per block
 constexpr int SQ_CHUNK = 16384, SQ_MOST = 1024;
+constexpr long long AW_BLOCKS = most_blocks(256), AW_ELEMENTS = AW_BLOCKS * AW_CHUNK;      // of a launch; of a tensor: its blocks fit one launch
 
 template <int TENSORS>
 struct Table32 {
@@ -288,12 +289,12 @@ bool aw_rows_ok(const long long* tensors, int n) {
     if (!tensors || n < 1) return false;
     for (int i = 0; i < n; ++i) {
         const long long* r = row(tensors, i);
-        if (r[7] < 0 || r[7] > (1ll << 42) || r[8] < W2C_F32 || r[8] > W2C_F16 || (r[7] && !r[1])) return false;
+        if (r[7] < 0 || r[7] > AW_ELEMENTS || r[8] < W2C_F32 || r[8] > W2C_F16 || (r[7] && !r[1])) return false;
     }
     return true;
 }
 
-// walks the tensors of one element type in launches of at most `most` tensors and 2^30 blocks; add(row, index, first block, blocks), flush(blocks)
+// walks the tensors of one element type in launches of at most `most` tensors and AW_BLOCKS blocks; add(row, index, first block, blocks), flush(blocks)
 template <typename Add, typename Flush>
 bool aw_batches(const long long* tensors, int n, int dtype, int most, long long chunk, Add add, Flush flush) {
     int count = 0;
@@ -302,7 +303,7 @@ bool aw_batches(const long long* tensors, int n, int dtype, int most, long long 
         const long long* r = row(tensors, i);
         if (r[8] != dtype || r[7] == 0) continue;
         const long long need = (r[7] + chunk - 1) / chunk;
-        if (count && (count == most || blocks + need > (1ll << 30))) {
+        if (count && (count == most || blocks + need > AW_BLOCKS)) {
             if (!flush(count, (int)blocks)) return false;
             count = 0;
             blocks = 0;

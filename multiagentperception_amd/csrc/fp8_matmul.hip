@@ -518,10 +518,10 @@ __global__ __launch_bounds__(256) void quantize_kernel(Quantize q) {
 }
 
 // out[c] = sum over the parts in order within 16 strips, then in strip order
-__global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict__ parts, long long n, long long cols, float* __restrict__ out) {
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict__ parts, long long n, long long cols, long long from, float* __restrict__ out) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, strip = threadIdx.x >> 6;
-    const long long c = (long long)blockIdx.x * 64 + lane;
+    const long long c = from + (long long)blockIdx.x * 64 + lane;
     float s = 0.f;
     if (c < cols)
         for (long long k = strip; k < n; k += 16) s += parts[k * cols + c];
@@ -573,6 +573,11 @@ Cut product_cut(int M, int N, int K) {
     return {128, 64, (int)parts};
 }
 
+long long product_blocks(int M, int N, int K) {
+    const Cut cut = product_cut(M, N, K);
+    return tiles(M, N, cut.tm, cut.tn);
+}
+
 template <typename T, bool FAST>
 int launch_product(const Product& p, hipStream_t st) {
     if (p.M <= ROWS_MOST) {
@@ -596,7 +601,7 @@ int launch_product(const Product& p, hipStream_t st) {
 }
 
 long long workspace_bytes_of(int M, int N, int K) {
-    if (M < 1 || N < 1 || K < KT || K % KT) return W2C_E_ARG;
+    if (M < 1 || N < 1 || K < KT || K % KT || M > 0x7FFFFFFF - 255 || N > 0x7FFFFFFF - 255) return W2C_E_ARG;
     const int parts = M <= ROWS_MOST ? 1 : product_cut(M, N, K).parts;
     return parts > 1 ? (long long)parts * M * N * (long long)sizeof(float) : 0;
 }
@@ -604,9 +609,10 @@ long long workspace_bytes_of(int M, int N, int K) {
 int product(bool fast, const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
             const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, void* stream) {
     if (!a || !a_scale || !b || !b_scale || !c || M < 1 || N < 1 || K < KT || K % KT || K > (1 << 22) || dtype < W2C_F32 || dtype > W2C_F16) return W2C_E_ARG;
+    if (M > 0x7FFFFFFF - 255 || N > 0x7FFFFFFF - 255) return W2C_E_ARG;                       // (sizes are rounded up to tiles)
     if ((a_tile != 1 && a_tile != 128) || (b_tile != 1 && b_tile != 128) || (long long)M * N > (1ll << 40)) return W2C_E_ARG;
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) return W2C_E_ARG;
-    if ((long long)((M + 127) / 128) * ((N + 127) / 128) > 0x7FFFFFFF) return W2C_E_ARG;
+    if (M <= ROWS_MOST ? tiles(1, N, 1, 16) > most_blocks(256) : product_blocks(M, N, K) > most_blocks(256)) return W2C_E_ARG;      // (one launch)
     w2c_clear_error();
     const long long need = workspace_bytes_of(M, N, K);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return W2C_E_ARG;
@@ -639,7 +645,7 @@ extern "C" long long w2c_quantize_fp8_workspace_bytes(long long rows, long long 
 extern "C" int w2c_quantize_fp8(const void* x, int dtype, long long rows, long long cols, long long stride, int tile, void* codes, void* scale,
                                 void* codes_t, void* scale_t, float* column_sums, void* workspace, long long workspace_bytes, void* stream) {
     if (!x || dtype < W2C_F32 || dtype > W2C_F16 || rows < 1 || cols < 1 || stride < cols || (tile != 1 && tile != 128)) return W2C_E_ARG;
-    if ((!codes && !codes_t && !column_sums) || (codes && !scale) || (codes_t && !scale_t) || rows > 65535ll * 128 || cols > (1ll << 31)) return W2C_E_ARG;
+    if ((!codes && !codes_t && !column_sums) || (codes && !scale) || (codes_t && !scale_t) || rows > 65535ll * 128 || cols > 128 * most_blocks(256)) return W2C_E_ARG;
     if (codes_t && (reinterpret_cast<uintptr_t>(codes_t) & 15)) return W2C_E_ARG;
     const bool parts = column_sums && w2c_quantize_fp8_workspace_bytes(rows, cols) > 0;
     if (parts && (!workspace || workspace_bytes < w2c_quantize_fp8_workspace_bytes(rows, cols))) return W2C_E_ARG;
@@ -651,7 +657,10 @@ extern "C" int w2c_quantize_fp8(const void* x, int dtype, long long rows, long l
     else if (dtype == W2C_BF16) hipLaunchKernelGGL((quantize_kernel<bf16_t>), grid, dim3(256), 0, st, q);
     else hipLaunchKernelGGL((quantize_kernel<f16_t>), grid, dim3(256), 0, st, q);
     if (parts)
-        hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, (const float*)workspace, (rows + 127) / 128, cols,
-                           column_sums);
+        for (long long from = 0; from < cols; from += 64 * most_blocks(1024)) {
+            const long long blocks = (cols - from + 63) / 64;
+            hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)(blocks < most_blocks(1024) ? blocks : most_blocks(1024))), dim3(1024), 0, st,
+                               (const float*)workspace, (rows + 127) / 128, cols, from, column_sums);
+        }
     return w2c_launch_status();
 }

@@ -361,10 +361,10 @@ __global__ __launch_bounds__(256) void ln_columns_kernel(const T* __restrict__ d
 
 // dw[c] = sum over the parts, in part order within each of 16 strips and then strip order (a fixed tree).  blockIdx.y: 0 = dw, 1 = db
 template <typename W>
-__global__ __launch_bounds__(1024) void ln_sum_parts_kernel(const float* __restrict__ parts, int n_parts, int D, W* __restrict__ dw, W* __restrict__ db) {
+__global__ __launch_bounds__(1024) void ln_sum_parts_kernel(const float* __restrict__ parts, int n_parts, int D, int from, W* __restrict__ dw, W* __restrict__ db) {
     __shared__ float red[16][64];
     W* out = blockIdx.y ? db : dw;
-    const int lane = threadIdx.x & 63, strip = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    const int lane = threadIdx.x & 63, strip = threadIdx.x >> 6, c = from + blockIdx.x * 64 + lane;
     float s = 0.f;
     if (out && c < D) {
         const float* p = parts + (long long)blockIdx.y * D + c;
@@ -444,11 +444,19 @@ int ln_backward(const void* dy, const void* h, const void* dh, long long rows, i
                                parts);
     }
 #undef LN_BWD
-    if (parts)
-        hipLaunchKernelGGL((ln_sum_parts_kernel<W>), dim3((D + 63) / 64, 2), dim3(1024), 0, st, (const float*)parts, nb, D, (W*)dw, (W*)db);
+    constexpr int MOST = (int)most_blocks(1024);
+    for (int from = 0; parts && from < D; from += 64 * MOST) {
+        const int blocks = (D - from + 63) / 64;
+        hipLaunchKernelGGL((ln_sum_parts_kernel<W>), dim3(blocks < MOST ? blocks : MOST, 2), dim3(1024), 0, st, (const float*)parts, nb, D, from, (W*)dw,
+                           (W*)db);
+    }
     return w2c_launch_status();
 }
 
+// rows of more than 16 384 columns take a block of 1024 threads each, in one launch
+bool ln_shape_ok(long long rows, int cols) {
+    return rows >= 1 && rows <= 0x7FFFFFFF && cols >= 1 && cols <= (1 << 30) && (cols <= 16384 || rows <= most_blocks(1024));
+}
 bool ln_types_ok(int dtype, int wtype) { return dtype >= W2C_F32 && dtype <= W2C_F16 && (wtype == W2C_F32 || wtype == dtype); }
 
 }  // namespace
@@ -456,7 +464,7 @@ bool ln_types_ok(int dtype, int wtype) { return dtype >= W2C_F32 && dtype <= W2C
 extern "C" int w2c_layer_norm_forward(const void* x, const void* residual, int dtype, long long rows, int cols, const void* weight, const void* bias,
                                       int wtype, float eps, void* y, void* h, float* mean, float* rstd, void* stream) {
     if (!x || !y || !mean || !rstd || (residual && !h) || !ln_types_ok(dtype, wtype)) return W2C_E_ARG;
-    if (rows < 1 || rows > 0x7FFFFFFF || cols < 1 || cols > (1 << 30)) return W2C_E_ARG;
+    if (!ln_shape_ok(rows, cols)) return W2C_E_ARG;
     w2c_clear_error();
     const hipStream_t st = (hipStream_t)stream;
 #define LN_CALL(T, W) return ln_forward<T, W>(x, residual, rows, cols, weight, bias, eps, y, h, mean, rstd, st)
@@ -471,7 +479,7 @@ extern "C" int w2c_layer_norm_forward(const void* x, const void* residual, int d
 }
 
 extern "C" long long w2c_layer_norm_workspace_bytes(long long rows, int cols, int dtype) {
-    if (rows < 1 || rows > 0x7FFFFFFF || cols < 1 || cols > (1 << 30) || dtype < W2C_F32 || dtype > W2C_F16) return W2C_E_ARG;
+    if (!ln_shape_ok(rows, cols) || dtype < W2C_F32 || dtype > W2C_F16) return W2C_E_ARG;
     return (long long)ln_backward_blocks(rows, cols) * 2 * cols * (long long)sizeof(float);
 }
 
@@ -479,7 +487,7 @@ extern "C" int w2c_layer_norm_backward(const void* dy, const void* h, const void
                                        int wtype, const float* mean, const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
                                        long long workspace_bytes, void* stream) {
     if (!dy || !h || !mean || !rstd || !dx || !ln_types_ok(dtype, wtype)) return W2C_E_ARG;
-    if (rows < 1 || rows > 0x7FFFFFFF || cols < 1 || cols > (1 << 30)) return W2C_E_ARG;
+    if (!ln_shape_ok(rows, cols)) return W2C_E_ARG;
     if ((dweight || dbias) && (!workspace || workspace_bytes < w2c_layer_norm_workspace_bytes(rows, cols, dtype))) return W2C_E_ARG;
     w2c_clear_error();
     const hipStream_t st = (hipStream_t)stream;

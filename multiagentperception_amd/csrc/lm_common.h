@@ -148,6 +148,9 @@ __device__ __forceinline__ float wave_max(float v) {
     }));
 }
 
+// A launch counts the work-items of a dimension in 32 bits: the most blocks of so many threads.
+constexpr long long most_blocks(int threads) { return 0xFFFFFFFFll / threads; }
+
 // Block scales are powers of two, held as a biased exponent byte (e8m0: value 2^(b - 127), 255 = NaN): the matrix instructions take them as
 // they are, and scaling by one is exact.  The scale of a block is the smallest 2^e with amax <= TOP * 2^e, by the fields of the two
 // floats; a block of zeros has 2^0.  amax has to be finite and >= 0.

@@ -249,10 +249,11 @@ __device__ __forceinline__ void sort_down(K (&k)[8]) {
 // taken k times.  Bound by instructions: 65536 x 500 bf16 without alternatives, with 2, 8 and 20:
 // 26, 44, 54 and 79 us, where a wave per row that is walked like longer ones takes 32, 63, 83 and 124.
 template <typename T, int A>
-__global__ __launch_bounds__(256) void lp_short_forward_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int per, Out o) {
+__global__ __launch_bounds__(256) void lp_short_forward_kernel(const T* __restrict__ x, long long from, long long rows, int C, long long row_stride, int per,
+                                                               Out o) {
     constexpr int VEC = ElemOf<T>::VEC, E = A * VEC, RW = 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = o.top;
-    const long long row0 = ((long long)blockIdx.x * 4 + wave) * per, row = row0 + lane;
+    const long long row0 = from + ((long long)blockIdx.x * 4 + wave) * per, row = row0 + lane;
     if (row0 >= rows) return;                            // whole waves
     const int n = rows - row0 < per ? (int)(rows - row0) : per;
     u32x4_t raw[RW][A];
@@ -476,13 +477,13 @@ __device__ __forceinline__ void walk_row(const T* __restrict__ p, int origin, in
 // parts == nullptr: the whole row is here.  Otherwise part blockIdx.y of it, and its (m, s, u) and k keys go to parts / part_keys
 // [row][part] for lp_join_kernel.
 template <typename T, int NW>
-__global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int part_len,
-                                                             Out o, float* __restrict__ parts, key_t* __restrict__ part_keys) {
+__global__ __launch_bounds__(256) void lp_row_forward_kernel(const T* __restrict__ x, long long from, long long rows, int C, long long row_stride,
+                                                             int part_len, Out o, float* __restrict__ parts, key_t* __restrict__ part_keys) {
     constexpr int VEC = ElemOf<T>::VEC, TPR = NW * 64, ROWS = 256 / TPR;
     extern __shared__ key_t shared[];                    // top_keys_words per row
     __shared__ float slots[3][NW];
     const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6, k = o.top;
-    const long long row = (long long)blockIdx.x * ROWS + (NW == 1 ? wave : 0);
+    const long long row = from + (long long)blockIdx.x * ROWS + (NW == 1 ? wave : 0);
     if (row >= rows) return;                             // whole waves, and only where no barrier follows
     const T* p = x + row * row_stride;
     const int lo = blockIdx.y * part_len, hi = C - lo < part_len ? C : lo + part_len;
@@ -700,11 +701,11 @@ __global__ __launch_bounds__(256) void lp_lane_backward_kernel(const T* __restri
 // a block (NW = 4) or a wave (NW = 1) per part of a row; the places of the target and of the alternatives get more than that, and are written again
 // by the first wave of the block that wrote them
 template <typename T, int NW>
-__global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restrict__ x, long long rows, int C, long long row_stride, int part_len,
-                                                              Grad g, T* __restrict__ dx) {
+__global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restrict__ x, long long from, long long rows, int C, long long row_stride,
+                                                              int part_len, Grad g, T* __restrict__ dx) {
     constexpr int VEC = ElemOf<T>::VEC, TPR = NW * 64, ROWS = 256 / TPR;
     const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const long long row = (long long)blockIdx.x * ROWS + (NW == 1 ? threadIdx.x >> 6 : 0);
+    const long long row = from + (long long)blockIdx.x * ROWS + (NW == 1 ? threadIdx.x >> 6 : 0);
     if (row >= rows) return;
     const T* p = x + row * row_stride;
     T* d = dx + row * C;
@@ -750,6 +751,15 @@ int lp_part_len(int C, int n) {                // a multiple of 8 elements
     const long long len = ((long long)C + n - 1) / n;
     return (int)((len + 7) / 8 * 8);
 }
+// launch(first row, blocks) over all rows, in as many launches as the limit on a launch's work-items makes of them
+template <typename F>
+void lp_launches(long long rows, int per_block, F launch) {
+    const long long most = most_blocks(256) * per_block;
+    for (long long from = 0; from < rows; from += most) {
+        const long long n = rows - from < most ? rows - from : most;
+        launch(from, (unsigned)((n + per_block - 1) / per_block));
+    }
+}
 bool lp_lane(int C, long long inner) { return inner > 1 || C <= LP_LANE_MOST; }
 
 struct LaneGrid {
@@ -784,24 +794,29 @@ int lp_forward(const void* x, long long outer, int C, long long inner, long long
     constexpr int VEC = ElemOf<T>::VEC, MOST = 8 / VEC;                  // eight values a lane
     if (C + VEC - 1 <= 64 * VEC * MOST) {
         const int per = outer >= 4 * 4096 ? 4 : outer >= 4096 ? 2 : 1;   // as many waves as the card holds before rows share one
-        const dim3 grid((unsigned)((outer + 4 * per - 1) / (4 * per)));
-        if (C + VEC - 1 <= 64 * VEC)
-            hipLaunchKernelGGL((lp_short_forward_kernel<T, 1>), grid, dim3(256), 0, st, (const T*)x, outer, C, row_stride, per, o);
-        else
-            hipLaunchKernelGGL((lp_short_forward_kernel<T, MOST>), grid, dim3(256), 0, st, (const T*)x, outer, C, row_stride, per, o);
+        lp_launches(outer, 4 * per, [&](long long from, unsigned blocks) {
+            if (C + VEC - 1 <= 64 * VEC)
+                hipLaunchKernelGGL((lp_short_forward_kernel<T, 1>), dim3(blocks), dim3(256), 0, st, (const T*)x, from, outer, C, row_stride, per, o);
+            else
+                hipLaunchKernelGGL((lp_short_forward_kernel<T, MOST>), dim3(blocks), dim3(256), 0, st, (const T*)x, from, outer, C, row_stride, per, o);
+        });
         return w2c_launch_status();
     }
     if (C <= LP_WAVE_MOST) {
-        hipLaunchKernelGGL((lp_row_forward_kernel<T, 1>), dim3((unsigned)((outer + 3) / 4)), dim3(256), (size_t)(k ? 4 * top_keys_words<1>(k) * sizeof(key_t) : 0), st,
-                           (const T*)x, outer, C, row_stride, C, o, (float*)nullptr, (key_t*)nullptr);
+        lp_launches(outer, 4, [&](long long from, unsigned blocks) {
+            hipLaunchKernelGGL((lp_row_forward_kernel<T, 1>), dim3(blocks), dim3(256), (size_t)(k ? 4 * top_keys_words<1>(k) * sizeof(key_t) : 0), st,
+                               (const T*)x, from, outer, C, row_stride, C, o, (float*)nullptr, (key_t*)nullptr);
+        });
         return w2c_launch_status();
     }
     const int n = lp_parts(outer, C);
     const int len = n > 1 ? lp_part_len(C, n) : C, used = (int)(((long long)C + len - 1) / len);
     key_t* keys = n > 1 ? (key_t*)ws : nullptr;
     float* parts = n > 1 ? (float*)(keys + (long long)outer * n * k) : nullptr;
-    hipLaunchKernelGGL((lp_row_forward_kernel<T, 4>), dim3((unsigned)outer, used), dim3(256), (size_t)(k ? top_keys_words<4>(k) * sizeof(key_t) : 0), st,
-                       (const T*)x, outer, C, row_stride, len, o, parts, keys);
+    lp_launches(outer, 1, [&](long long from, unsigned blocks) {
+        hipLaunchKernelGGL((lp_row_forward_kernel<T, 4>), dim3(blocks, used), dim3(256), (size_t)(k ? top_keys_words<4>(k) * sizeof(key_t) : 0), st,
+                           (const T*)x, from, outer, C, row_stride, len, o, parts, keys);
+    });
     if (n > 1)
         hipLaunchKernelGGL((lp_join_kernel<T>), dim3((unsigned)((outer + 3) / 4)), dim3(256), 0, st, (const T*)x, outer, C, row_stride, used, o,
                            (const float*)parts, (const key_t*)keys);
@@ -826,8 +841,9 @@ int lp_backward(const void* x, long long outer, int C, long long inner, long lon
         return w2c_launch_status();
     }
     if (C <= LP_WAVE_MOST) {
-        hipLaunchKernelGGL((lp_row_backward_kernel<T, 1>), dim3((unsigned)((outer + 3) / 4)), dim3(256), 0, st, (const T*)x, outer, C, row_stride, C, g,
-                           (T*)dx);
+        lp_launches(outer, 4, [&](long long from, unsigned blocks) {
+            hipLaunchKernelGGL((lp_row_backward_kernel<T, 1>), dim3(blocks), dim3(256), 0, st, (const T*)x, from, outer, C, row_stride, C, g, (T*)dx);
+        });
         return w2c_launch_status();
     }
     // a block per row, or per part of one where there are not rows enough for two rounds of blocks; at least four accesses per lane
@@ -835,8 +851,10 @@ int lp_backward(const void* x, long long outer, int C, long long inner, long lon
     const long long most = (C + 256 * ElemOf<T>::VEC * 4 - 1) / (256 * ElemOf<T>::VEC * 4);
     if (n > most) n = most;
     const int len = lp_part_len(C, (int)n);
-    hipLaunchKernelGGL((lp_row_backward_kernel<T, 4>), dim3((unsigned)outer, (C - 1) / len + 1), dim3(256), 0, st, (const T*)x, outer, C, row_stride,
-                       len, g, (T*)dx);
+    lp_launches(outer, 1, [&](long long from, unsigned blocks) {
+        hipLaunchKernelGGL((lp_row_backward_kernel<T, 4>), dim3(blocks, (C - 1) / len + 1), dim3(256), 0, st, (const T*)x, from, outer, C, row_stride,
+                           len, g, (T*)dx);
+    });
     return w2c_launch_status();
 }
 

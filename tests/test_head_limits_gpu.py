@@ -1,0 +1,67 @@
+"""The head's operators on more rows or columns than one launch has work-items for (2^32): the parts of the work at the seams and at the end have the bits that
+the same call answers for a view of them alone."""
+import pytest
+import torch
+
+from multiagentperception_amd import ops
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _give_back():
+    yield
+    torch.cuda.empty_cache()
+
+
+# 16 rows to a block of the short rows' forward, 4 to one of their backward and of both up to 2 048 classes, 1 beyond
+@pytest.mark.parametrize("rows,classes,seam", [((1 << 28) + 5, 65, 16 * (0xFFFFFFFF // 256)), ((1 << 26) + 9, 513, 4 * (0xFFFFFFFF // 256)), ((1 << 24) + 3, 2049, 0xFFFFFFFF // 256)])
+def test_log_probs_of_many_rows(rows, classes, seam):
+    n = 1100
+    x = torch.zeros(rows, classes, dtype=BF16, device="cuda")
+    target = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    assert rows - n < seam < rows                                 # (views of 1 024 rows and more: fewer rows of 2 049 classes are split into parts and joined)
+    places = [slice(0, n), slice(rows - n, rows)] + ([slice((1 << 26) - n, (1 << 26) + 7)] if rows > 1 << 27 else [])
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    for s in places:
+        x[s] = torch.randn(x[s].shape, generator=g, device="cuda").to(BF16)
+        target[s] = torch.randint(0, classes, target[s].shape, generator=g, device="cuda")
+    ones = torch.ones(rows, device="cuda")
+    r = ops.log_probs_forward(x, target, 2)
+    d = ops.log_probs_backward(x, target, r, ones, ones)
+    for s in places:
+        p = ops.log_probs_forward(x[s], target[s], 2)
+        for a, b in zip(r, p):
+            assert torch.equal(a[s], b)
+        assert torch.equal(d[s], ops.log_probs_backward(x[s], target[s], p, ones[s], ones[s]))
+    some = slice(rows // 2, rows // 2 + 4)                        # zeros: every class alike
+    assert torch.equal(r.top_index[some], torch.tensor([[0, 1]] * 4, device="cuda")) and not d[some][:, 1:].isnan().any()
+
+
+def test_weight_gradients_of_a_norm_over_many_columns():
+    D = (1 << 28) + 77
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = (torch.randn(1, D, generator=g, device="cuda") for _ in range(2))
+    w = torch.ones(D, device="cuda")
+    y, h, mean, rstd = ops.layer_norm_forward(x, w)
+    dw, db = ops.layer_norm_backward(dy, h, w, mean, rstd)[1:]
+    assert torch.equal(db, dy[0])                                 # one row: no sum
+    for s in (slice(0, 100), slice(64 * (0xFFFFFFFF // 1024) - 50, 64 * (0xFFFFFFFF // 1024) + 50), slice(D - 100, D)):
+        want = dy[0, s].double() * (x[0, s].double() - mean.double()) * rstd.double()
+        assert ((dw[s].double() - want).abs() <= 4 * 2.0 ** -24 * (dy[0, s].double() * rstd.double()).abs() * (x[0, s].double().abs() + mean.double().abs())).all()
+
+
+def test_column_sums_of_many_columns():
+    rows, cols = 129, (1 << 28) + 200                              # two tiles of rows: the sums are joined by a second launch
+    x = torch.zeros(rows, cols, dtype=BF16, device="cuda")
+    seam = 64 * (0xFFFFFFFF // 1024)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    places = (slice(0, 300), slice(seam - 300, seam + 300), slice(cols - 300, cols))
+    for s in places:
+        x[:, s] = torch.randn(x[:, s].shape, generator=g, device="cuda").to(BF16)
+    sums = ops.quantize_fp8(x, rows=False, sums=True).sums
+    for s in places:
+        v = x[:, s].double()
+        assert ((sums[s].double() - v.sum(0)).abs() <= 130 * 2.0 ** -24 * v.abs().sum(0)).all()
+    assert not sums[300:seam - 300].any()
