@@ -554,7 +554,7 @@ int w2c_adamw_step(const long long* tensors, int n, int state_bits, double lr, c
                    long long workspace_bytes, w2c_stream_t stream);
 
 /* 8-bit product with a power-of-two scale per 128 of the reduction: c[m][n] = sum_k a[m][k] 2^(sa - 127) b[n][k] 2^(sb - 127) (+ bias[n]), c [M, N] of
- * dtype.  a [M, K], b [N, K]: e4m3fn codes, rows padded with zero codes to K, a multiple of 128, 16-byte aligned; a_scale e8m0
+ * dtype.  a [M, K], b [N, K]: e4m3fn codes, rows padded with zero codes to K, a multiple of 128 up to 8 388 480, 16-byte aligned; a_scale e8m0
  * [a_tile = 1: M | 128: ceil(M / 128)][K / 128], b_scale alike: a scale per row or per 128 rows.  The products are exact and
  * added in f32 (a code times its scale goes in as a bf16 number: infinite beyond f32's range, a multiple of 2^-133); deterministic.  workspace: w2c_matmul_fp8_workspace_bytes (0: none),
  * 16-byte aligned.
@@ -570,7 +570,7 @@ int w2c_matmul_fp8_fast(const void* a, const void* a_scale, int a_tile, const vo
  * with tile 128][ceil(cols / 128)]), of the transposed x (codes_t [cols, rows padded to 128], 16-byte aligned, scale_t alike), either NULL if not
  * wanted, from one read.  A scale is the smallest power of two with amax <= 448 * scale, amax over the block's finite values (1 for zeros);
  * codes round to nearest even; values that are not finite become NaN.  column_sums: f32 [cols] = sums of x over its rows, or NULL (with it:
- * workspace of w2c_quantize_fp8_workspace_bytes, 0: none). */
+ * workspace of w2c_quantize_fp8_workspace_bytes, 0: none).  rows <= 8 388 480, the longest reduction of w2c_matmul_fp8; cols < 2^31 - 128. */
 long long w2c_quantize_fp8_workspace_bytes(long long rows, long long cols);
 int w2c_quantize_fp8(const void* x, int dtype, long long rows, long long cols, long long stride, int tile, void* codes, void* scale, void* codes_t,
                      void* scale_t, float* column_sums, void* workspace, long long workspace_bytes, w2c_stream_t stream);

@@ -22,6 +22,9 @@ namespace {
 
 typedef unsigned char u8;
 constexpr int KT = 128;                       // elements of the reduction per scale
+// The longest reduction is the most rows that the quantiser takes (its tiles of rows are a grid's second dimension): a gradient of weights sums over them.
+// 256 rows of it are 2^31 bytes at most, within a descriptor and its 32-bit offsets.
+constexpr int ROW_TILES = 65535, K_MOST = ROW_TILES * KT;
 // The row kernel reads all of a once per 16 columns: against 16384 x 8192 weights it takes 27 us with 3 rows, 40 with 17, 46 with 24 and 52 with 32, the tile
 // kernels 42 to 46 with any of 17 to 64; against 1024 x 8192 it is 12 and 13 with 24 rows.
 constexpr int ROWS_MOST = 24;
@@ -608,7 +611,7 @@ long long workspace_bytes_of(int M, int N, int K) {
 
 int product(bool fast, const void* a, const void* a_scale, int a_tile, const void* b, const void* b_scale, int b_tile, int M, int N, int K,
             const float* bias, void* c, int dtype, void* workspace, long long workspace_bytes, void* stream) {
-    if (!a || !a_scale || !b || !b_scale || !c || M < 1 || N < 1 || K < KT || K % KT || K > (1 << 22) || dtype < W2C_F32 || dtype > W2C_F16) return W2C_E_ARG;
+    if (!a || !a_scale || !b || !b_scale || !c || M < 1 || N < 1 || K < KT || K % KT || K > K_MOST || dtype < W2C_F32 || dtype > W2C_F16) return W2C_E_ARG;
     if (M > 0x7FFFFFFF - 255 || N > 0x7FFFFFFF - 255) return W2C_E_ARG;                       // (sizes are rounded up to tiles)
     if ((a_tile != 1 && a_tile != 128) || (b_tile != 1 && b_tile != 128) || (long long)M * N > (1ll << 40)) return W2C_E_ARG;
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) return W2C_E_ARG;
@@ -645,7 +648,7 @@ extern "C" long long w2c_quantize_fp8_workspace_bytes(long long rows, long long 
 extern "C" int w2c_quantize_fp8(const void* x, int dtype, long long rows, long long cols, long long stride, int tile, void* codes, void* scale,
                                 void* codes_t, void* scale_t, float* column_sums, void* workspace, long long workspace_bytes, void* stream) {
     if (!x || dtype < W2C_F32 || dtype > W2C_F16 || rows < 1 || cols < 1 || stride < cols || (tile != 1 && tile != 128)) return W2C_E_ARG;
-    if ((!codes && !codes_t && !column_sums) || (codes && !scale) || (codes_t && !scale_t) || rows > 65535ll * 128 || cols > 128 * most_blocks(256)) return W2C_E_ARG;
+    if ((!codes && !codes_t && !column_sums) || (codes && !scale) || (codes_t && !scale_t) || rows > K_MOST || cols > 128 * most_blocks(256)) return W2C_E_ARG;
     if (codes_t && (reinterpret_cast<uintptr_t>(codes_t) & 15)) return W2C_E_ARG;
     const bool parts = column_sums && w2c_quantize_fp8_workspace_bytes(rows, cols) > 0;
     if (parts && (!workspace || workspace_bytes < w2c_quantize_fp8_workspace_bytes(rows, cols))) return W2C_E_ARG;

@@ -2116,6 +2116,7 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
 
 
 FP8_BLOCK = 128                    # elements of the reduction that share a scale in matmul_fp8
+FP8_MOST = 65535 * FP8_BLOCK       # rows of a quantised matrix, and so the longest reduction
 
 
 class Fp8Blocks(typing.NamedTuple):
@@ -2139,7 +2140,7 @@ def _fp8_new(rows, cols, tile, dev):
 
 def quantize_fp8(x, tile=1, rows=True, columns=False, sums=False):
     """x f32 / bf16 / f16 [R, C] (its rows may be those of a wider tensor) -> Fp8Quantized: x by rows (to multiply along C), the transposed x (to
-    multiply along R), and x's column sums f32 [C], each if wanted, from one read.  tile 1: a scale per row's 128 elements; 128: per 128 x 128
+    multiply along R), and x's column sums f32 [C], each if wanted, from one read; R at most FP8_MOST.  tile 1: a scale per row's 128 elements; 128: per 128 x 128
     tile, so that both forms hold the same values (weights).  include/w2c_hip.h w2c_quantize_fp8."""
     if not x.is_cuda:
         _need_gpu(x)
@@ -2151,6 +2152,8 @@ def quantize_fp8(x, tile=1, rows=True, columns=False, sums=False):
     if not (rows or columns or sums):
         raise W2CError("quantize_fp8: nothing wanted")
     R, C = x.shape
+    if R > FP8_MOST:
+        raise W2CError("quantize_fp8: at most %d rows, got %d" % (FP8_MOST, R))
     by_rows = _fp8_new(R, C, tile, dev) if rows else None
     by_cols = _fp8_new(C, R, tile, dev) if columns else None
     total = torch.empty(C, dtype=torch.float32, device=dev) if sums else None
@@ -2188,6 +2191,8 @@ def matmul_fp8(a, b, bias=None, out_dtype=BF16, fast=False):
     (M, K), (N, Kb) = a.codes.shape, b.codes.shape
     if K != Kb or a.cols != b.cols:
         raise W2CError("matmul_fp8: %d against %d columns" % (a.cols, b.cols))
+    if K > FP8_MOST:
+        raise W2CError("matmul_fp8: at most %d columns, got %d" % (FP8_MOST, K))
     if out_dtype not in _ELEM:
         raise W2CError("matmul_fp8: f32, bf16 or f16 output expected, got %s" % out_dtype)
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,)):

@@ -428,8 +428,8 @@ class _LinearFp8Fn(torch.autograd.Function):
 def linear_fp8(x, weight, bias=None, fast=False):
     """y [..., N] = x [..., K] W^T + bias with the product (and, under autograd, both products of its backward) of 8-bit operands with a power-of-two
     scale per 128 elements of the sum.  weight: [N, K] f32 / bf16 / f16, or ops.Fp8Blocks of it (quantize_fp8(weight, 128).rows: laid out once,
-    for inference).  fast: ops.matmul_fp8's, for the products with a 16-bit result (a gradient of f32 weights is not one).  HIP kernels under the
-    "hip" backend on GPU tensors, F.linear otherwise."""
+    for inference).  fast: ops.matmul_fp8's, for the products with a 16-bit result (a gradient of f32 weights is not one).  At most
+    ops.FP8_MOST rows, inputs and outputs.  HIP kernels under the "hip" backend on GPU tensors, F.linear otherwise."""
     if isinstance(weight, ops.Fp8Blocks):
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise ops.W2CError("linear_fp8: quantised weights are for inference; pass the weights themselves to differentiate")

@@ -3,7 +3,8 @@ the same call answers for a view of them alone."""
 import pytest
 import torch
 
-from multiagentperception_amd import ops
+from multiagentperception_amd import ops, train_ops
+from multiagentperception_amd._native import W2CError
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -65,3 +66,36 @@ def test_column_sums_of_many_columns():
         v = x[:, s].double()
         assert ((sums[s].double() - v.sum(0)).abs() <= 130 * 2.0 ** -24 * v.abs().sum(0)).all()
     assert not sums[300:seam - 300].any()
+
+
+@pytest.mark.parametrize("rows", [(1 << 22) + 1, ops.FP8_MOST])
+def test_a_linear_step_over_as_many_rows_as_its_forward_takes(rows):
+    """the gradient of the weights is a sum over all rows; 300 of them are not zero, so that many roundings at most"""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, dy = torch.zeros(rows, 16, device="cuda"), torch.zeros(rows, 24, device="cuda")
+    at = torch.randint(0, rows, (300,), generator=g, device="cuda")
+    at[0] = rows - 1
+    x[at], dy[at] = torch.randn(300, 16, generator=g, device="cuda"), torch.randn(300, 24, generator=g, device="cuda")
+    x.requires_grad_()
+    w = torch.randn(24, 16, generator=g, device="cuda", requires_grad=True)
+    y = train_ops.linear_fp8(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    held = lambda t: t.codes[:, :rows].float().double() * t.scale.float().double().repeat_interleave(128, 1)[:, :rows]       # noqa: E731
+    a, b = (held(ops.quantize_fp8(t.detach(), rows=False, columns=True).columns)[:, at.unique()] for t in (dy, x))
+    assert ((dw.double() - a @ b.t()).abs() <= 301 * 2.0 ** -24 * (a.abs() @ b.abs().t())).all() and dw.any()
+    some = at.sort()[0][-20:]
+    by_rows = lambda t, tile: (t.codes.float().double() * t.scale.float().double().repeat_interleave(tile, 0)[:t.codes.shape[0]])[:, :t.cols]       # noqa: E731
+    qw = ops.quantize_fp8(w.detach(), 128, columns=True)
+    for got, left, right in ((y, x, qw.rows), (dx, dy, qw.columns)):               # one block of 128 either way
+        p, q = by_rows(ops.quantize_fp8(left.detach()[some]).rows, 1), by_rows(right, 128)
+        assert ((got.detach()[some].double() - p @ q.t()).abs() <= 25 * 2.0 ** -24 * (p.abs() @ q.abs().t())).all()
+
+
+def test_more_rows_are_refused_by_the_forward():
+    x = torch.zeros(ops.FP8_MOST + 1, 16, device="cuda", requires_grad=True)
+    with pytest.raises(W2CError, match="at most"):
+        train_ops.linear_fp8(x, torch.zeros(24, 16, device="cuda"))
+    c = torch.zeros(2, ops.FP8_MOST + 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    q = ops.Fp8Blocks(c, torch.zeros(2, c.shape[1] // 128, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu), c.shape[1])
+    with pytest.raises(W2CError, match="at most"):
+        ops.matmul_fp8(q, q)
