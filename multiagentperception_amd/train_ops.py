@@ -402,7 +402,9 @@ class _LinearFp8Fn(torch.autograd.Function):
         wq = ops.quantize_fp8(weight.detach().contiguous(), ops.FP8_BLOCK, columns=need_x)
         y = ops.matmul_fp8(xq.rows, wq.rows, None if bias is None else bias.detach().float().contiguous(), x.dtype, fast)
         ctx.fast = fast
-        ctx.x_columns, ctx.w_columns = xq.columns, wq.columns
+        # (by autograd, so that hooks of saved tensors see them and a backward frees them)
+        ctx.save_for_backward(*(t for q in (xq.columns, wq.columns) for t in ((None, None) if q is None else (q.codes, q.scale))))
+        ctx.cols = rows.shape[0], weight.shape[0]
         ctx.shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
         return y.view(x.shape[:-1] + (weight.shape[0],))
 
@@ -410,14 +412,15 @@ class _LinearFp8Fn(torch.autograd.Function):
     def backward(ctx, dy):
         ops.first_order_only("linear_fp8")
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        x_codes, x_scale, w_codes, w_scale = ctx.saved_tensors
         rows = dy.reshape(-1, dy.shape[-1])
         q = ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous(), 1, rows=need_x, columns=need_w, sums=need_b)
         dx = dw = db = None
         if need_x:
-            dx = ops.matmul_fp8(q.rows, ctx.w_columns, None, ctx.dtypes[0], ctx.fast).view(ctx.shape)
+            dx = ops.matmul_fp8(q.rows, ops.Fp8Blocks(w_codes, w_scale, ctx.cols[1]), None, ctx.dtypes[0], ctx.fast).view(ctx.shape)
         if need_w:
             if rows.shape[0]:
-                dw = ops.matmul_fp8(q.columns, ctx.x_columns, None, ctx.dtypes[1], ctx.fast)
+                dw = ops.matmul_fp8(q.columns, ops.Fp8Blocks(x_codes, x_scale, ctx.cols[0]), None, ctx.dtypes[1], ctx.fast)
             else:
                 dw = torch.zeros((dy.shape[-1], ctx.shape[-1]), dtype=ctx.dtypes[1], device=dy.device)
         if need_b:
