@@ -395,8 +395,9 @@ class _LinearFp8Fn(torch.autograd.Function):
     is summed over, W with a scale per 128 x 128 tile.  Every operand is read once and quantised both ways from that read."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, fast):
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+    def forward(ctx, x, weight, bias, fast, differentiated):
+        # (a parameter needs its gradient under no_grad too, as far as needs_input_grad goes: the caller knows whether there will be a backward)
+        need_x, need_w = (differentiated and need for need in ctx.needs_input_grad[:2])
         rows = x.reshape(-1, x.shape[-1])
         xq = ops.quantize_fp8(rows if rows.is_contiguous() else rows.contiguous(), 1, columns=need_w)
         wq = ops.quantize_fp8(weight.detach().contiguous(), ops.FP8_BLOCK, columns=need_x)
@@ -425,7 +426,7 @@ class _LinearFp8Fn(torch.autograd.Function):
                 dw = torch.zeros((dy.shape[-1], ctx.shape[-1]), dtype=ctx.dtypes[1], device=dy.device)
         if need_b:
             db = q.sums.to(ctx.dtypes[2])
-        return dx, dw, db, None
+        return dx, dw, db, None, None
 
 
 def linear_fp8(x, weight, bias=None, fast=False):
@@ -445,7 +446,7 @@ def linear_fp8(x, weight, bias=None, fast=False):
     if _backend == "hip" and x.is_cuda:
         if weight.dim() != 2 or not weight.numel() or weight.shape[1] != x.shape[-1] or (bias is not None and tuple(bias.shape) != (weight.shape[0],)):
             raise ops.W2CError("linear_fp8: x %s, weight %s and bias do not fit" % (tuple(x.shape), tuple(weight.shape)))
-        return _LinearFp8Fn.apply(x, weight, bias, fast)
+        return _LinearFp8Fn.apply(x, weight, bias, fast, torch.is_grad_enabled())
     return F.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
 
 

@@ -3,7 +3,7 @@ import pytest
 import torch
 import torch.utils.checkpoint
 
-from multiagentperception_amd import train_ops
+from multiagentperception_amd import ops, train_ops
 
 pytestmark = pytest.mark.gpu
 F8 = (torch.float8_e4m3fn, torch.float8_e8m0fnu)
@@ -78,3 +78,21 @@ def test_frozen_parts_are_not_kept():
     with hooks():
         y = m(x)
     assert len(seen) == 2 and torch.autograd.grad(y, x, dy)[0].any()                       # the transposed weights alone
+
+
+def test_without_gradients_nothing_is_transposed(monkeypatch):
+    m, x, dy = _layer()
+    asked, real = [], ops.quantize_fp8
+
+    def spy(t, tile=1, rows=True, columns=False, sums=False):
+        asked.append((rows, columns, sums))
+        return real(t, tile, rows, columns, sums)
+
+    monkeypatch.setattr(ops, "quantize_fp8", spy)
+    y = m(x)
+    assert asked == [(True, True, False)] * 2
+    asked.clear()
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            assert torch.equal(m(x), y)
+    assert asked == [(True, False, False)] * 4
