@@ -13,7 +13,8 @@ class AdamW(torch.optim.Optimizer):
     state_bits 32: f32 moments; 8: moments in 8 bits (ops.adamw_step: e4m3 with a power-of-two scale per 256 elements, rounded at random by
     `seed`), 2 bytes an element in place of 8.  max_norm: all groups' gradients together are scaled down to this norm; `last_norm` is the
     norm before that (f32 on the device).  lr: a number (a schedule may change it between eager steps) or an f32 device tensor of one
-    element, which captured steps follow.  A parameter without a gradient is left out of the step."""
+    element, which captured steps follow.  A parameter without a gradient is left out of the step.  eps may be 0: an element that has had no
+    gradient (none whose square f32 holds) is then only decayed."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None, seed=0):
         if state_bits not in (8, 32):
