@@ -585,8 +585,11 @@ template <typename T, bool FAST>
 int launch_product(const Product& p, hipStream_t st) {
     if (p.M <= ROWS_MOST) {
         const dim3 grid((p.N + 15) / 16);
-        // 16 waves to a block where 4 would leave the card without enough of them
-        const bool few = p.N < 16 * 768 && p.K >= 16 * KT;
+        // 16 waves to a block of 16 columns where there is at most one block for a CU and each of the waves still gets a few k blocks to keep on their
+        // way; they pay for their larger sum.  4 / 16 waves, us, bf16, with 1 row: 4096 x 6144 7.9 / 7.6, 4096 x 8192 11.9 / 8.7, 512 x 16384 16.3 / 12.2, but
+        // 4096 x 4096 7.0 / 7.9, 8192 x 4096 8.9 / 12.8, 6144 x 12288 22.5 / 24.4; with 16 rows: 4096 x 6144 8.8 / 9.5, 4096 x 7168 12.0 / 10.3,
+        // 4096 x 8192 12.8 / 11.2, 6144 x 7168 18.3 / 18.6, and the worst on this side, 512 x 12288 14.5 / 16.2.
+        const bool few = p.N <= 16 * 256 && p.K >= 56 * KT;
 #define MATMUL_ROWS(MT)                                                                                                             \
     do {                                                                                                                            \
         if (few) hipLaunchKernelGGL((matmul_rows_kernel<T, FAST, MT, 16>), grid, dim3(1024), 0, st, p);                                    \
