@@ -558,20 +558,23 @@ int launch_tile(const Product& p, hipStream_t st) {
 
 long long tiles(int M, int N, int tm, int tn) { return (long long)((M + tm - 1) / tm) * ((N + tn - 1) / tn); }
 // What a product of the tile kernels is cut into: the largest tiles of which there are enough for the 256 CUs (a larger tile reads less per product),
-// and where there are at most half as many of the smallest, parts of the reduction: about 256 in all, each long enough to be worth the sum of the
-// parts (8 blocks of 128; 16 with more than 64 tiles, which already draw most of what the L2s give).  To bf16, with 8 / as it is / with 24 blocks at least:
-// 256 x 256 x 4096 9.3 / 9.3 / 11.2 us, 64 x 4096 x 4096 12.4 / 12.4 / 13.2, 1024 x 1024 x 2048 15.3 / 10.6 / 10.6; 512 parts instead of 256
-// take 1024 x 1024 x 4096 from 16.7 to 20.5 us and 512 x 512 x 8192 from 14.8 to 19.8.
+// and where there are at most half as many of the smallest, parts of the reduction: about 256 in all, none shorter than 8 blocks of 128 (16 with more
+// than 64 tiles), to be worth the sum of the parts.  us to bf16, default / FAST:
+//   256 x 256 or 128 x 128 tiles  3200 x 3200 x 4096 (169 of the former) 85 or 83; 3584 x 3584 x 4096 (196) 90 or 107 / 55 or 73
+//   128 x 128 or 128 x 64 tiles   1536 x 1920 x 4096 (180) 34 or 34 / 21 or 28; 1664 x 2048 x 4096 (208) 36 or 38 / 22 or 30
+//   1 or 2 parts, up to 64 tiles  512 x 512 x 1152 8.5 or 9.7 / 7.0 or 8.9; 256 x 256 x 1920 (15 blocks) 11.5 or 10.4 / 9.0 either way
+//   ... with more                 1024 x 1024 x 2176 12.8 or 16.6 / 9.8 or 14.8; 1024 x 1024 x 4096 21.6 or 19.4
+//   about 256 parts, or twice     64 x 4096 x 4096 13.1 or 16.3, 512 x 512 x 8192 15.5 or 20.3
 struct Cut {
     int tm, tn, parts;
 };
 Cut product_cut(int M, int N, int K) {
     if (tiles(M, N, 256, 256) >= 160) return {256, 256, 1};
-    if (tiles(M, N, 128, 128) >= 224) return {128, 128, 1};
+    if (tiles(M, N, 128, 128) >= 180) return {128, 128, 1};
     const long long t = tiles(M, N, 128, 64);
     long long parts = t > 128 ? 1 : 256 / t;
-    const int least = t > 64 ? 16 : 8, most = (K / KT + least - 1) / least;
-    if (parts > most) parts = most;
+    const int least = t > 64 ? 16 : 8, most = K / KT / least;
+    if (parts > most) parts = most > 1 ? most : 1;
     if (parts > 16) parts = 16;
     return {128, 64, (int)parts};
 }
