@@ -10,7 +10,7 @@
 //
 // HBM-bound: one read forward, one read and one write backward.  Three shapes of work:
 //   lane per row   class dimension strided (label maps) or at most 64 classes: 64 neighbouring rows per wave, alternatives in registers
-//   wave per row   up to 2 048 contiguous classes; a wave for up to four rows that fit its registers (about 500 classes)
+//   wave per row   up to 2 048 contiguous classes; a wave for one or two rows that fit its registers (about 500 classes)
 //   block per row or per part of a row   longer; few long rows are split over blocks and joined by a second launch
 // Alternatives of the last two: every thread keeps the largest (value, index) of what it read; the k-th largest of those is a bound that
 // at most k threads reach, and only their values are looked through again.
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256) void lp_lane_forward_kernel(const T* __restric
     }
 }
 
-// ---- up to four short rows per wave ------------------------------------------------------------------------------------------------------
+// ---- one or two short rows per wave ------------------------------------------------------------------------------------------------------
 template <typename K>
 __device__ __forceinline__ void order_pair(K& a, K& b) {
     const K x = a, y = b;
@@ -244,14 +244,14 @@ __device__ __forceinline__ void sort_down(K (&k)[8]) {
     order_pair(k[0], k[4]), order_pair(k[1], k[5]), order_pair(k[2], k[6]), order_pair(k[3], k[7]);
     order_pair(k[2], k[4]), order_pair(k[3], k[5]), order_pair(k[1], k[2]), order_pair(k[3], k[4]), order_pair(k[5], k[6]);
 }
-// Rows of at most A accesses of 16 bytes a lane stay in registers, and `per` of them (up to four) share a wave: their loads are in flight together, and the
+// Rows of at most A accesses of 16 bytes a lane stay in registers, and `per` of them (one or two) share a wave: their loads are in flight together, and the
 // closing arithmetic of each is done by a lane of its own, at once.  Alternatives: every lane sorts its values, the largest of the lanes' first ones is
-// taken k times.  Bound by instructions: 65536 x 500 bf16 without alternatives, with 2, 8 and 20:
-// 26, 44, 54 and 79 us, where a wave per row that is walked like longer ones takes 32, 63, 83 and 124.
+// taken k times.  Bound by instructions: 65536 x 500 bf16 without alternatives, with 2, 8 and 20: 24, 38, 49 and 72 us, where a wave per row that is
+// walked like longer ones takes 32, 63, 83 and 124.
 template <typename T, int A>
 __global__ __launch_bounds__(256) void lp_short_forward_kernel(const T* __restrict__ x, long long from, long long rows, int C, long long row_stride, int per,
                                                                Out o) {
-    constexpr int VEC = ElemOf<T>::VEC, E = A * VEC, RW = 4;
+    constexpr int VEC = ElemOf<T>::VEC, E = A * VEC, RW = 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = o.top;
     const long long row0 = from + ((long long)blockIdx.x * 4 + wave) * per, row = row0 + lane;
     if (row0 >= rows) return;                            // whole waves
@@ -739,7 +739,7 @@ __global__ __launch_bounds__(256) void lp_row_backward_kernel(const T* __restric
     if (here) d[j] = from_f32<T>(v);                                   // (the same place: the same value)
 }
 
-// few long rows: enough parts for about four blocks on every CU, none under 256 lanes' accesses of 16 bytes
+// few long rows: enough parts for about four blocks on every CU, of at least 1 024 classes (2 049 make two parts: 8 rows 5.7 us, of 4 096 5.5)
 int lp_parts(long long rows, int C) {
     if (C <= LP_WAVE_MOST) return 1;
     long long n = (1024 + rows - 1) / rows;
@@ -793,7 +793,9 @@ int lp_forward(const void* x, long long outer, int C, long long inner, long long
     const int k = o.top;
     constexpr int VEC = ElemOf<T>::VEC, MOST = 8 / VEC;                  // eight values a lane
     if (C + VEC - 1 <= 64 * VEC * MOST) {
-        const int per = outer >= 4 * 4096 ? 4 : outer >= 4096 ? 2 : 1;   // as many waves as the card holds before rows share one
+        const int per = outer >= 8192 ? 2 : 1;
+        // (the card holds 8 192 waves.  1 / 2 rows to a wave, us, bf16, without / with 8 alternatives: 4096 x 250 4.2 or 4.4 / 6.2 or 7.0, 8192 x 250 5.5 or 5.2 /
+        // 9.3 or 9.6, 16384 x 250 7.8 or 6.9 / 14.9 either way, 65536 x 500 23.4 or 22.5 / 47.7 or 48.0; with four 22.9 / 50.0)
         lp_launches(outer, 4 * per, [&](long long from, unsigned blocks) {
             if (C + VEC - 1 <= 64 * VEC)
                 hipLaunchKernelGGL((lp_short_forward_kernel<T, 1>), dim3(blocks), dim3(256), 0, st, (const T*)x, from, outer, C, row_stride, per, o);
@@ -846,7 +848,7 @@ int lp_backward(const void* x, long long outer, int C, long long inner, long lon
         });
         return w2c_launch_status();
     }
-    // a block per row, or per part of one where there are not rows enough for two rounds of blocks; at least four accesses per lane
+    // a block per row, or per part of one where there are not rows enough for two rounds of blocks; more than two accesses per lane
     long long n = (4096 + outer - 1) / outer;
     const long long most = (C + 256 * ElemOf<T>::VEC * 4 - 1) / (256 * ElemOf<T>::VEC * 4);
     if (n > most) n = most;
