@@ -540,7 +540,7 @@ int w2c_log_probs_backward(const void* x, int dtype, long long outer, int classe
  * addresses but the last two; p and g of dtype; step f32 [1], the number of steps done, advanced by the call.
  *   state_bits 32: m, v f32 [elements] (first and second moment), the two scales unused
  *   state_bits  8: m, v e4m3 codes of the first moment and of the ROOT of the second, m_scale / v_scale e8m0 [ceil(elements / 256)]; rounded up
- *                  or down at random by a hash of (seed, step, place); codes of values that are not finite are NaN
+ *                  or down at random by a hash of (seed, step, place in the tensor); codes of values that are not finite are NaN
  * eps may be 0: an element whose root of the second moment is 0 then (in f32) is only decayed.
  * lr: lr_dev[0] (f32) where lr_dev is not NULL, so that a captured step follows it.  n_squares > 0: the gradients are scaled by
  * min(1, max_norm / (norm + 1e-6)), norm = sqrt(sum of squares), written to `norm` (f32 [1]) unless NULL; squares come from

@@ -11,8 +11,9 @@
 //
 // 8-bit moments: m and r = sqrt(v) (the root halves the range to cover) as e4m3 codes, 256 elements to a power-of-two scale.  b2 = 0.999 moves v by
 // a thousandth of itself per step, far less than half a step of any 8-bit code: rounded to nearest, v would never decay.  So both are
-// rounded up or down at random with the distance as the chance (the mean is kept, a value that did not move keeps its code); the random bits are a
-// hash of (seed, t, place), so a step gives the same bits every time.  A root above 0 keeps a code above 0: m / r stays bounded.  The step
+// rounded up or down at random with the distance as the chance (the mean of m and of the root is kept, v's grows by the root's variance: some per cent of
+// what b2 = 0.999 takes off it in a step; a value that did not move keeps its code).  The random bits are a hash of (seed, t, place), so a step
+// gives the same bits every time, and tensors of one call are rounded alike at the same place.  A root above 0 keeps a code above 0: m / r stays bounded.  The step
 // itself uses m and v before they are rounded.  Codes of values that are not finite are NaN; the scale comes from the others.
 #include "lm_common.h"
 

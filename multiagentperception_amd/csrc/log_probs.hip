@@ -23,6 +23,8 @@ constexpr float LP_FLOOR = -200.f;            // exp(-200) is 0 in f32: stands f
 constexpr int LP_TOP_MOST = 32, LP_SPLIT_MOST = 64;
 constexpr int LP_LANE_MOST = 64, LP_WAVE_MOST = 2048;      // classes
 
+// exp(d): the hardware's 2^x of the rounded d log2(e).  That rounding is half a step of f32 of the argument, |d| 2^-24 of the result, beside the
+// instruction's own step: d = 10 below the row's largest, a term is off by 6e-7 of itself and adds 3e-11 of the sum.
 __device__ __forceinline__ float exp_d(float d) { return __builtin_amdgcn_exp2f(d * LP_L2E); }
 
 struct Run {                                  // of the values seen so far

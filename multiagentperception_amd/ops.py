@@ -2051,7 +2051,7 @@ def adamw_step(params, grads, states, steps, lr=1e-3, beta1=0.9, beta2=0.999, ep
     params f32 / bf16 / f16 with gradients of their types; steps: one f32 element each, advanced by the call; states, all alike:
       (m, v)                    f32, laid out like the parameter
       (m, m_scale, v, v_scale)  8 bits: m and the ROOT of v as float8_e4m3fn of the parameter's elements in memory order, float8_e8m0fnu
-                                scales of ADAMW_STATE_BLOCK elements; rounded at random by (seed, step, place)
+                                scales of ADAMW_STATE_BLOCK elements; rounded at random by (seed, step, place in the tensor)
     lr: a number, or an f32 device tensor of one element (a captured step then follows it).  max_norm: the gradients are scaled down to this
     norm in all; `squares` (grad_squares) where more tensors than these share the norm.  -> the norm before that (f32 on the device), or None."""
     dev, p, g, sizes, types, plain = _adamw_tensors(params, grads)
