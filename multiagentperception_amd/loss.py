@@ -200,13 +200,18 @@ def log_probs(input, target=None, top=0, dim=-1, ignore_index=-100):
     """Log probability of `target` under the softmax of `input` along `dim`, the entropy, and the `top` largest log probabilities with their
     classes (largest first, equal logits by the lower class), all differentiable but the classes.  input: logits (f32, bf16, f16), target:
     integers of the other dimensions, `ignore_index` there answers 0.  -inf is a masked class; a row of nothing else answers logp = -inf, entropy 0
-    and has no gradient.  A target outside [0, n_classes) that is not `ignore_index` answers NaN.  Pixels of label maps: dim=1."""
+    and has no gradient.  A target outside [0, n_classes) that is not `ignore_index` answers NaN and
+    has no number for its row's gradient.  Pixels of label maps: dim=1."""
     if target is not None:
         target = target.long().contiguous()
     if input.is_cuda:
         rows = input.dim() == 2 and dim % 2 == 1 and input.stride(1) == 1 and input.stride(0) >= input.shape[1]
         return LogProbs(*_LogProbsFn.apply(input if rows else input.contiguous(), target, int(top), int(dim), int(ignore_index)))
+    if not -input.dim() <= dim < input.dim():
+        raise ops.W2CError("log_probs: dim %d of a %d-dimensional tensor" % (dim, input.dim()))
     x = input.float().movedim(dim, -1)
+    if target is not None and target.shape != x.shape[:-1]:
+        raise ops.W2CError("log_probs: target must have the shape %s" % (tuple(x.shape[:-1]),))
     if not 0 <= top <= min(x.shape[-1], ops.LOG_PROBS_TOP_MOST):
         raise ops.W2CError("log_probs: top must lie in 0 .. min(classes, %d), got %d of %d classes" % (ops.LOG_PROBS_TOP_MOST, top, x.shape[-1]))
     empty = (x == -float("inf")).all(-1, keepdim=True)
@@ -217,7 +222,9 @@ def log_probs(input, target=None, top=0, dim=-1, ignore_index=-100):
     if target is not None:
         inside = (target >= 0) & (target < x.shape[-1])
         logp = lp.gather(-1, target.masked_fill(~inside, 0).unsqueeze(-1)).squeeze(-1)
-        logp = logp.masked_fill(~inside, float("nan")).masked_fill(target == ignore_index, 0.0)
+        ignored = target == ignore_index
+        # (a factor, not a fill: the gradient of such a row is NaN too)
+        logp = (logp * torch.ones_like(logp).masked_fill(~inside & ~ignored, float("nan"))).masked_fill(ignored, 0.0)
     if top:
         top_index = x.masked_fill(x.isnan(), -float("inf")).sort(dim=-1, descending=True, stable=True)[1][..., :top]
         top_logp = lp.gather(-1, top_index)
