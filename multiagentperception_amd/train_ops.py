@@ -452,6 +452,7 @@ def linear_fp8(x, weight, bias=None, fast=False):
 
 class LinearFp8(nn.Linear):
     """nn.Linear (same parameters, same state_dict keys) on linear_fp8(); `fast` is linear_fp8's"""
+    fast = False                                     # (of modules that were pickled without it)
 
     def __init__(self, in_features, out_features, bias=True, device=None, dtype=None, fast=False):
         super().__init__(in_features, out_features, bias, device, dtype)
