@@ -25,8 +25,9 @@ constexpr int KT = 128;                       // elements of the reduction per s
 // The longest reduction is the most rows that the quantiser takes (its tiles of rows are a grid's second dimension): a gradient of weights sums over them.
 // 256 rows of it are 2^31 bytes at most, within a descriptor and its 32-bit offsets.
 constexpr int ROW_TILES = 65535, K_MOST = ROW_TILES * KT;
-// The row kernel reads all of a once per 16 columns: against 16384 x 8192 weights it takes 27 us with 3 rows, 40 with 17, 46 with 24 and 52 with 32, the tile
-// kernels 42 to 46 with any of 17 to 64; against 1024 x 8192 it is 12 and 13 with 24 rows.
+// The row kernel reads all of a once per 16 columns, the tile kernels multiply 128 rows whatever there are.  us to bf16, row / tile kernels: 16384 x 8192
+// weights with 16 rows 35.6 / 40.2, 20 41.4 / 38.4, 24 44.8 / 38.9, 32 50.8 / 39.3; 1024 x 8192 with 16 10.2 / 12.0, 24 13.0 / 12.2, 32 14.5 / 12.2; 4096 x 4096
+// with 16 9.2 / 11.3, 24 10.7 / 11.5, 32 11.8 / 11.9.
 constexpr int ROWS_MOST = 24;
 
 // four scale bytes (k blocks kb .. kb + 3) of a row; bytes past the row's end are not read, and not used
