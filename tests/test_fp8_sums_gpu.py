@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
-# one wave to a row block and four, both row kernels; then the three tiles; rows of scales that are whole dwords and others; reductions in parts
+# up to 24 rows, blocks of 4 and of 16 waves; then the three tiles; rows of scales that are whole dwords and others; reductions in parts
 SHAPES = [(1, 33, 512), (16, 100, 640), (17, 257, 128), (24, 40, 4100), (5, 50, 2048), (1, 4096, 8192), (9, 120, 7200), (24, 40, 8200), (25, 65, 1500), (130, 259, 512), (40, 100, 8192), (33, 65, 8200), (1000, 700, 4096),
           (1900, 1910, 384), (1900, 1910, 512), (3300, 3200, 384), (3300, 3200, 512)]
 
